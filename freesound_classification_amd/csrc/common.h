@@ -13,6 +13,10 @@ int l16_fwd_clock(double* shader_mhz);      // conv_l16.hip: shader clock of the
 
 inline hipStream_t as_stream(fsc_stream_t s) { return reinterpret_cast<hipStream_t>(s); }
 
+// Clears `bytes` (a multiple of 4) at `p` with a kernel.  Not hipMemsetAsync: every entry point may be recorded into a HIP graph, and
+// memset nodes of a replayed graph have left wrong values behind.
+hipError_t zero_async(void* p, size_t bytes, hipStream_t st);      // misc.hip
+
 // Development switches (FSC_* environment variables), read ONCE when the first entry point needs them -- never on the per-call path.
 struct EnvFlags {
     bool no_l16, no_l16_pool, no_l16_wgrad, l16_no_xcd, l16_vec1, dbg_noksplit, frontend_generic, fe_block_sync;

@@ -2524,8 +2524,8 @@ int launch_fwd_cot(const FwdPlan& p, const float* in, const float* packed, const
     dim3 grid((unsigned)p.grid_x, p.co_blocks, p.g.ksplit);
     if (p.g.ksplit > 1 && !accumulate) {
         const size_t bytes = sizeof(float) * (size_t)p.g.n * p.g.cout * p.g.hw;
-        hipError_t e = hipMemsetAsync(out, 0, bytes, st);
-        FSC_CHECK_ARG(e == hipSuccess, "fsc_conv_fwd: memset failed: %s", hipGetErrorString(e));
+        hipError_t e = fsc::zero_async(out, bytes, st);
+        FSC_CHECK_ARG(e == hipSuccess, "fsc_conv_fwd: clearing failed: %s", hipGetErrorString(e));
     }
     if (p.x3) {
         grid.x = (unsigned)p.launch_x;
@@ -2556,8 +2556,8 @@ int launch_fwd_wide(const FwdPlan& p, const float* in, const float* packed, cons
         dim3 grid((unsigned)p.launch_x, 1, p.g.ksplit);
         if (p.g.ksplit > 1 && !accumulate) {
             const size_t bytes = sizeof(float) * (size_t)p.g.n * p.g.cout * p.g.hw;
-            hipError_t e = hipMemsetAsync(out, 0, bytes, st);
-            FSC_CHECK_ARG(e == hipSuccess, "fsc_conv_fwd: memset failed: %s", hipGetErrorString(e));
+            hipError_t e = fsc::zero_async(out, bytes, st);
+            FSC_CHECK_ARG(e == hipSuccess, "fsc_conv_fwd: clearing failed: %s", hipGetErrorString(e));
         }
         if constexpr (COT == 10) {
             if (p.pt == 2) {
@@ -2600,8 +2600,8 @@ int launch_amax(const float* x, long n, float* out, hipStream_t st, int slots) {
     if (blocks == 1 && slots == 1) {
         hipLaunchKernelGGL(amax_kernel, dim3(1), dim3(256), 0, st, x, n, out, 1, 1);
     } else {
-        hipError_t e = hipMemsetAsync(out, 0, sizeof(float) * (slots == 1 ? 1 : fsc::kAmaxFloats), st);
-        FSC_CHECK_ARG(e == hipSuccess, "fsc_amax: memset failed: %s", hipGetErrorString(e));
+        hipError_t e = fsc::zero_async(out, sizeof(float) * (slots == 1 ? 1 : fsc::kAmaxFloats), st);
+        FSC_CHECK_ARG(e == hipSuccess, "fsc_amax: clearing failed: %s", hipGetErrorString(e));
         hipLaunchKernelGGL(amax_kernel, dim3((unsigned)blocks), dim3(256), 0, st, x, n, out, 0, slots);
     }
     FSC_LAUNCH_CHECK("fsc_amax");

@@ -172,8 +172,8 @@ int run_gemm(const GemmArgs& g_in, hipStream_t st, const char* name) {
         if (ks > 16) ks = 16;
         if (ks > 1) {
             g.ksplit = (int)ks;
-            hipError_t e = hipMemsetAsync(g.c, 0, sizeof(float) * (size_t)g.m * g.n, st);
-            FSC_CHECK_ARG(e == hipSuccess, "%s: memset failed: %s", name, hipGetErrorString(e));
+            hipError_t e = fsc::zero_async(g.c, sizeof(float) * (size_t)g.m * g.n, st);
+            FSC_CHECK_ARG(e == hipSuccess, "%s: clearing failed: %s", name, hipGetErrorString(e));
         }
     }
     grid.z = g.ksplit;

@@ -225,8 +225,8 @@ int fsc_bce_fwd(const float* logits, const float* targets, float* loss_scalar, d
                 fsc_stream_t stream) {
     FSC_CHECK_ARG(logits && targets && loss_scalar && workspace && count > 0, "fsc_bce_fwd: bad arguments");
     hipStream_t st = fsc::as_stream(stream);
-    hipError_t e = hipMemsetAsync(workspace, 0, sizeof(double), st);
-    FSC_CHECK_ARG(e == hipSuccess, "fsc_bce_fwd: memset failed: %s", hipGetErrorString(e));
+    hipError_t e = fsc::zero_async(workspace, sizeof(double), st);
+    FSC_CHECK_ARG(e == hipSuccess, "fsc_bce_fwd: clearing failed: %s", hipGetErrorString(e));
     hipLaunchKernelGGL(bce_fwd_kernel, dim3(grid_for(count) > 256 ? 256 : grid_for(count)), dim3(256), 0, st, logits,
                        targets, workspace, count);
     hipLaunchKernelGGL(bce_finish_kernel, dim3(1), dim3(1), 0, st, workspace, loss_scalar, count);

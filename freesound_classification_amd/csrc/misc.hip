@@ -304,6 +304,16 @@ __global__ __launch_bounds__(256) void first_block_1d_kernel(const float* __rest
 
 }  // namespace
 
+namespace fsc {
+
+hipError_t zero_async(void* p, size_t bytes, hipStream_t st) {
+    const long count = (long)(bytes / sizeof(float));
+    if (count > 0) hipLaunchKernelGGL(fill_kernel, dim3(grid_for(count)), dim3(256), 0, st, reinterpret_cast<float*>(p), 0.f, count);
+    return hipPeekAtLastError();
+}
+
+}  // namespace fsc
+
 extern "C" {
 
 int fsc_first_block_1d_finish(const float* dwx, const float* dc, const float* dc_chan_sum, const float* mean, const float* invstd,

@@ -1866,8 +1866,8 @@ size_t fsc_bn_workspace_ticket_offset(int c) { return part_doubles(c) * sizeof(d
 
 int fsc_bn_workspace_reset(void* workspace, int c, fsc_stream_t stream) {
     FSC_CHECK_ARG(workspace && c > 0, "fsc_bn_workspace_reset: bad arguments");
-    hipError_t e = hipMemsetAsync(carve(workspace, c).tickets, 0, (size_t)c * sizeof(unsigned), fsc::as_stream(stream));
-    FSC_CHECK_ARG(e == hipSuccess, "fsc_bn_workspace_reset: memset failed: %s", hipGetErrorString(e));
+    hipError_t e = fsc::zero_async(carve(workspace, c).tickets, (size_t)c * sizeof(unsigned), fsc::as_stream(stream));
+    FSC_CHECK_ARG(e == hipSuccess, "fsc_bn_workspace_reset: clearing failed: %s", hipGetErrorString(e));
     return 0;
 }
 
@@ -2079,8 +2079,8 @@ int fsc_bn_act_fwd_limbs(const float* x, const float* residual, const float* sca
         return 0;
     }
     if (y_amax) {
-        hipError_t e = hipMemsetAsync(y_amax, 0, fsc::kAmaxFloats * sizeof(float), st);
-        FSC_CHECK_ARG(e == hipSuccess, "fsc_bn_act_fwd: memset failed: %s", hipGetErrorString(e));
+        hipError_t e = fsc::zero_async(y_amax, fsc::kAmaxFloats * sizeof(float), st);
+        FSC_CHECK_ARG(e == hipSuccess, "fsc_bn_act_fwd: clearing failed: %s", hipGetErrorString(e));
     }
     const long total = (long)n * c * hw;
     if (hw >= 512) {

@@ -235,9 +235,9 @@ int fsc_layernorm_bwd(const float* dy, const float* x, const float* mean, const 
     FSC_CHECK_ARG(dy && x && mean && rstd && gamma && dx && dgamma && dbeta && rows > 0 && c > 0, "fsc_layernorm_bwd: bad arguments");
     hipStream_t st = fsc::as_stream(stream);
     hipLaunchKernelGGL(layernorm_bwd_kernel, dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, st, dy, x, mean, rstd, gamma, dx, rows, c);
-    hipError_t e = hipMemsetAsync(dgamma, 0, sizeof(float) * c, st);
-    if (e == hipSuccess) e = hipMemsetAsync(dbeta, 0, sizeof(float) * c, st);
-    FSC_CHECK_ARG(e == hipSuccess, "fsc_layernorm_bwd: memset failed: %s", hipGetErrorString(e));
+    hipError_t e = fsc::zero_async(dgamma, sizeof(float) * c, st);
+    if (e == hipSuccess) e = fsc::zero_async(dbeta, sizeof(float) * c, st);
+    FSC_CHECK_ARG(e == hipSuccess, "fsc_layernorm_bwd: clearing failed: %s", hipGetErrorString(e));
     long gy = (rows + 63) / 64;
     if (gy > 256) gy = 256;
     hipLaunchKernelGGL(layernorm_param_grad_kernel, dim3(fsc::ceil_div(c, 256), (unsigned)gy), dim3(256), 0, st, dy, x, mean, rstd,
