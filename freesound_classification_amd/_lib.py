@@ -32,6 +32,26 @@ class OptTensor(C.Structure):
                 ("state1", C.c_void_p), ("state2", C.c_void_p), ("count", C.c_long)]
 
 
+def _args_struct(name, ints, fields):
+    """A *_args structure of the C ABI: `ints`, then `fields` in the header's order -- "p:" pointers, "l:" element strides."""
+    kinds = {"p": C.c_void_p, "l": C.c_long}
+    listed = [(f, C.c_int) for f in ints.split()]
+    for part in fields.split():
+        kind, names = part.split(":")
+        listed += [(f, kinds[kind]) for f in names.split(",")]
+    return type(name, (C.Structure,), {"_fields_": listed})
+
+
+CausalConvArgs = _args_struct(
+    "CausalConvArgs", "batch length channels taps dtype silu",
+    "p:x l:x_batch,x_time p:weight,bias,lengths,initial,y,final,dy l:dy_batch,dy_time p:dfinal,dx,dinitial,dweight,dbias,workspace")
+ScanArgs = _args_struct(
+    "ScanArgs", "batch length channels states groups dtype softplus",
+    "p:u,dt,z,b,c l:u_batch,u_time,dt_batch,dt_time,z_batch,z_time,b_batch,b_time,b_group,c_batch,c_time,c_group "
+    "p:a_log,d,dt_bias,lengths,initial,y,final,checkpoints,workspace,dy l:dy_batch,dy_time "
+    "p:dfinal,du,ddt,dz,db,dc,da_log,dd,ddt_bias,dinitial")
+
+
 _P, _I, _L, _F, _SZ = C.c_void_p, C.c_int, C.c_long, C.c_float, C.c_size_t
 _U64 = C.c_uint64
 _D = C.POINTER(ConvDesc)
@@ -139,6 +159,17 @@ SIGNATURES = {
     "fsc_adam_step_factors": (None, [_F, _F, _F, _I, C.POINTER(C.c_float)]),
     "fsc_adam_amsgrad_step_dev": (_I, [C.POINTER(OptTensor), _I, _P, _F, _F, _F, _F, _F, _P]),
     "fsc_sgd_nesterov_step": (_I, [C.POINTER(OptTensor), _I, _F, _F, _F, _I, _F, _P]),
+    "fsc_causal_conv_fwd": (_I, [_P, _P]),
+    "fsc_causal_conv_bwd_workspace_bytes": (_SZ, [_P]),
+    "fsc_causal_conv_bwd": (_I, [_P, _P]),
+    "fsc_causal_conv_step": (_I, [_P, _P]),
+    "fsc_selective_scan_checkpoint_bytes": (_SZ, [_P]),
+    "fsc_selective_scan_workspace_bytes": (_SZ, [_P, _I]),
+    "fsc_selective_scan_fwd": (_I, [_P, _P]),
+    "fsc_selective_scan_bwd": (_I, [_P, _P]),
+    "fsc_selective_scan_step": (_I, [_P, _P]),
+    "fsc_adamw_step_factors": (None, [C.c_double, C.c_double, C.c_double, C.c_double, _L, C.POINTER(C.c_float)]),
+    "fsc_adamw_step": (_I, [_P, _I, _I, _I, _P, _P, C.c_double, C.c_double, _F, _F, _P]),
     "fsc_plane_border_sums": (_I, [_P, _I, _I, _I, _I, _P, _P]),
     "fsc_first_block_1d_finish": (_I, [_P] * 8 + [_I, _I, _I, _I, _P, _P, _P, _P]),
     "fsc_fill": (_I, [_P, _F, _L, _P]),

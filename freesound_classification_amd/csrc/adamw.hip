@@ -1,0 +1,243 @@
+// AdamW over many tensors.  Per element, in this order and with every product and sum rounded to fp32 by itself (no contraction: what is
+// held in 8 bits changes with the last bit, and a plain evaluation of the same formulas then holds the same bits):
+//   g = grad * grad_scale;  m = m beta1 + g (1 - beta1);  v = v beta2 + (g g)(1 - beta2);  r = sqrt(v)
+//   p = p decay - (m / (r inv_root + eps)) step_size
+// Bound: HBM.  32-bit moments: 28 bytes a parameter in fp32 (p, g, m, v read; p, m, v written); 8-bit moments: 16.
+//
+// 8-bit moments.  m and r = sqrt(v) (half the decades of v) are held as e4m3 values of x / scale, scale = the largest |x| of 256
+// consecutive elements / 448.  Rounding to nearest would freeze them: beta2 = 0.999 moves v by 0.1 % a step and half a step of e4m3 is
+// 6 %.  So a value is rounded down or up with the probability of its remainder, from 16 bits of a hash of (salt, step, element): the mean
+// moves as in 32 bits.  r > 0 is never held as 0 -- its next step would divide by eps.
+// One wave owns a block of 256: four elements a lane, the block's maximum through lane exchanges, no LDS.
+#include <math.h>
+
+#include "seq.h"
+
+namespace {
+
+constexpr int kBatch = 52;       // tensors per launch: 52 x 64 bytes of the 4 KB of kernel arguments
+constexpr int kChunk = 4096;     // elements per workgroup: 16 blocks of 256, four per wave
+constexpr int kThreads = 256;
+constexpr int kBlock = 256;
+constexpr float kTop = 448.0f;   // the largest e4m3 value
+
+struct Table {
+    fsc_adamw_tensor t[kBatch];
+    int chunk_start[kBatch + 1];
+    int n;
+};
+struct Hyper {
+    float decay, step_size, inv_root, step;
+    float beta1, rest1, beta2, rest2, eps, grad_scale;
+    const float* dev;            // non-null: the first four come from device memory
+};
+static_assert(sizeof(Table) + sizeof(Hyper) <= 4096, "kernel arguments");
+
+__device__ __forceinline__ uint32_t mix32(uint32_t x) {
+    x = (x ^ (x >> 16)) * 0x9E3779B9u;
+    x = (x ^ (x >> 15)) * 0xB7E15163u;
+    return x ^ (x >> 16);
+}
+
+// scale and 448 / top of a block (0 and 0 where the scale would be below the normal numbers: the block is held as zeros)
+struct BlockScale {
+    float scale, inverse;
+    __device__ explicit BlockScale(float top) {
+#pragma clang fp contract(off)
+        scale = top * (1.0f / kTop);
+        const bool dead = scale < 1.17549435e-38f;
+        inverse = dead ? 0.f : (1.0f / top) * kTop;
+        scale = dead ? 0.f : scale;
+    }
+};
+
+// e4m3 pattern of x * inverse, rounded down or up by the 16 random bits.  Normal values: adding them below the three mantissa bits
+// carries with the probability of the remainder; below 2^-6 the values are multiples of 2^-9.
+__device__ __forceinline__ uint32_t held(float x, float inverse, uint32_t bits16, bool keep_positive) {
+#pragma clang fp contract(off)
+    const float y = x * inverse, size = fabsf(y);
+    const uint32_t pattern = __float_as_uint(size);
+    const uint32_t normal = ((pattern + (bits16 << 4)) >> 20) - (120u << 3);
+    const uint32_t small = (uint32_t)(size * 512.0f + (float)bits16 * 0x1p-16f);
+    uint32_t code = size >= 0x1p-6f ? normal : small;
+    code = code > 0x7Eu ? 0x7Eu : code;
+    if (keep_positive && code == 0 && y > 0.f) code = 1;
+    return pattern < 0x7F800000u ? code | ((__float_as_uint(y) >> 24) & 0x80u) : 0x7Fu;
+}
+
+__device__ __forceinline__ float e4m3_value(uint32_t code) {
+    // exact by construction: sign, four exponent bits (bias 7), three mantissa bits; 0x7F / 0xFF = NaN
+    return __builtin_amdgcn_cvt_f32_fp8((int)code, 0);
+}
+
+template <typename T, int BITS>
+__global__ __launch_bounds__(kThreads) void adamw_kernel(Table tb, Hyper h) {
+#pragma clang fp contract(off)
+    if (h.dev != nullptr) {
+        h.decay = h.dev[0];
+        h.step_size = h.dev[1];
+        h.inv_root = h.dev[2];
+        h.step = h.dev[3];
+    }
+    int lo = 0, hi = tb.n - 1;                               // the last tensor that begins at or before this chunk
+    while (lo < hi) {
+        const int mid = (lo + hi + 1) >> 1;
+        if ((int)blockIdx.x >= tb.chunk_start[mid]) lo = mid; else hi = mid - 1;
+    }
+    const fsc_adamw_tensor t = tb.t[lo];
+    const long base = (long)((int)blockIdx.x - tb.chunk_start[lo]) * kChunk;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    T* p_ = reinterpret_cast<T*>(t.param);
+    const T* g_ = reinterpret_cast<const T*>(t.grad);
+    constexpr size_t kStateAlign = BITS == 32 ? 16 : 4;
+    const bool wide_t = (((size_t)t.param | (size_t)t.grad) & (4 * sizeof(T) - 1)) == 0 &&
+                        (((size_t)t.state0 | (size_t)t.state1) & (kStateAlign - 1)) == 0;
+    uint32_t key = 0;
+    if constexpr (BITS == 8) {
+        key = mix32(mix32((uint32_t)t.salt) + (uint32_t)h.step);
+        if (base >> 32) key = mix32(key + (uint32_t)(base >> 32));
+    }
+#pragma unroll
+    for (int it = 0; it < kChunk / (4 * kThreads); ++it) {
+        const long block = base + (it * (kThreads / 64) + wave) * kBlock;
+        if (block >= t.count) return;                        // (a wave's blocks ascend)
+        const long e = block + 4 * lane;
+        const int have = e >= t.count ? 0 : t.count - e < 4 ? (int)(t.count - e) : 4;
+        const bool wide = wide_t && have == 4;
+        float p[4], g[4], m[4], v[4];
+        fsc::load_row<4>(p_ + e, wide, have, p);
+        fsc::load_row<4>(g_ + e, wide, have, g);
+        if constexpr (BITS == 32) {
+            fsc::load_row<4>(reinterpret_cast<const float*>(t.state0) + e, wide, have, m);
+            fsc::load_row<4>(reinterpret_cast<const float*>(t.state1) + e, wide, have, v);
+        } else {
+            const uint8_t* c0 = reinterpret_cast<const uint8_t*>(t.state0) + e;
+            const uint8_t* c1 = reinterpret_cast<const uint8_t*>(t.state1) + e;
+            const float s0 = t.scale0[block / kBlock], s1 = t.scale1[block / kBlock];
+            uint32_t w0 = 0, w1 = 0;
+            if (wide) {
+                w0 = *reinterpret_cast<const uint32_t*>(c0);
+                w1 = *reinterpret_cast<const uint32_t*>(c1);
+            } else {
+                for (int i = 0; i < have; ++i) {
+                    w0 |= (uint32_t)c0[i] << (8 * i);
+                    w1 |= (uint32_t)c1[i] << (8 * i);
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                m[i] = e4m3_value((w0 >> (8 * i)) & 0xFF) * s0;
+                const float r = e4m3_value((w1 >> (8 * i)) & 0xFF) * s1;
+                v[i] = r * r;
+            }
+        }
+        float r[4], top0 = 0.f, top1 = 0.f;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float gs = g[i] * h.grad_scale;
+            m[i] = m[i] * h.beta1 + gs * h.rest1;
+            v[i] = v[i] * h.beta2 + (gs * gs) * h.rest2;
+            r[i] = sqrtf(v[i]);
+            p[i] = p[i] * h.decay - (m[i] / (r[i] * h.inv_root + h.eps)) * h.step_size;
+            const float am = fabsf(m[i]);
+            top0 = fmaxf(top0, am < INFINITY && i < have ? am : 0.f);
+            top1 = fmaxf(top1, r[i] < INFINITY && i < have ? r[i] : 0.f);
+        }
+        fsc::store_row<4>(p_ + e, wide, have, p);
+        if constexpr (BITS == 32) {
+            fsc::store_row<4>(reinterpret_cast<float*>(t.state0) + e, wide, have, m);
+            fsc::store_row<4>(reinterpret_cast<float*>(t.state1) + e, wide, have, v);
+        } else {
+            const BlockScale b0(fsc::wave_top(top0)), b1(fsc::wave_top(top1));
+            uint32_t w0 = 0, w1 = 0;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const uint32_t bits = mix32((uint32_t)(e + i) ^ key);
+                w0 |= held(m[i], b0.inverse, bits >> 16, false) << (8 * i);
+                w1 |= held(r[i], b1.inverse, bits & 0xFFFFu, true) << (8 * i);
+            }
+            uint8_t* c0 = reinterpret_cast<uint8_t*>(t.state0) + e;
+            uint8_t* c1 = reinterpret_cast<uint8_t*>(t.state1) + e;
+            if (wide) {
+                *reinterpret_cast<uint32_t*>(c0) = w0;
+                *reinterpret_cast<uint32_t*>(c1) = w1;
+            } else {
+                for (int i = 0; i < have; ++i) {
+                    c0[i] = (uint8_t)(w0 >> (8 * i));
+                    c1[i] = (uint8_t)(w1 >> (8 * i));
+                }
+            }
+            if (lane == 0) {
+                t.scale0[block / kBlock] = b0.scale;
+                t.scale1[block / kBlock] = b1.scale;
+            }
+        }
+    }
+}
+
+}  // namespace
+
+extern "C" {
+
+void fsc_adamw_step_factors(double lr, double beta1, double beta2, double weight_decay, long step, float* out4_host) {
+    out4_host[0] = (float)(1.0 - lr * weight_decay);
+    out4_host[1] = (float)(lr / (1.0 - pow(beta1, (double)step)));
+    out4_host[2] = (float)(1.0 / sqrt(1.0 - pow(beta2, (double)step)));
+    out4_host[3] = (float)(step & 0xFFFFFF);
+}
+
+int fsc_adamw_step(const fsc_adamw_tensor* tensors_host, int n_tensors, int dtype, int state_bits, const float* factors4,
+                   const float* factors4_dev, double beta1, double beta2, float eps, float grad_scale, fsc_stream_t stream) {
+    FSC_CHECK_ARG(tensors_host && n_tensors > 0 && (factors4 != nullptr) != (factors4_dev != nullptr), "fsc_adamw_step: bad arguments");
+    FSC_CHECK_ARG(fsc::dtype_ok(dtype), "fsc_adamw_step: dtype %d", dtype);
+    FSC_CHECK_ARG(state_bits == 32 || state_bits == 8, "fsc_adamw_step: state_bits %d (32 or 8)", state_bits);
+    for (int i = 0; i < n_tensors; ++i) {
+        const fsc_adamw_tensor& t = tensors_host[i];
+        FSC_CHECK_ARG(t.count >= 0, "fsc_adamw_step: tensor %d has %ld elements", i, t.count);
+        FSC_CHECK_ARG(t.count == 0 || (t.param && t.grad && t.state0 && t.state1), "fsc_adamw_step: tensor %d has null pointers", i);
+        FSC_CHECK_ARG(t.count == 0 || state_bits == 32 || (t.scale0 && t.scale1), "fsc_adamw_step: tensor %d misses its scales", i);
+        FSC_CHECK_ARG(t.count <= (long)kChunk * 0x3FFFFFFF, "fsc_adamw_step: tensor %d is too large", i);
+    }
+    Hyper h{};
+    if (factors4 != nullptr) {
+        h.decay = factors4[0];
+        h.step_size = factors4[1];
+        h.inv_root = factors4[2];
+        h.step = factors4[3];
+    }
+    h.beta1 = (float)beta1;
+    h.rest1 = (float)(1.0 - beta1);
+    h.beta2 = (float)beta2;
+    h.rest2 = (float)(1.0 - beta2);
+    h.eps = eps;
+    h.grad_scale = grad_scale;
+    h.dev = factors4_dev;
+    hipStream_t st = fsc::as_stream(stream);
+    int next = 0;
+    while (next < n_tensors) {
+        Table tb{};
+        long chunks = 0;
+        while (next < n_tensors && tb.n < kBatch) {
+            const fsc_adamw_tensor& t = tensors_host[next];
+            const long more = (t.count + kChunk - 1) / kChunk;
+            if (tb.n > 0 && chunks + more > 0x3FFFFFFF) break;
+            ++next;
+            if (more == 0) continue;
+            tb.t[tb.n] = t;
+            tb.chunk_start[tb.n++] = (int)chunks;
+            chunks += more;
+        }
+        if (tb.n == 0) continue;
+        tb.chunk_start[tb.n] = (int)chunks;
+        auto launch = [&](auto type) {
+            using T = decltype(type);
+            if (state_bits == 32) hipLaunchKernelGGL((adamw_kernel<T, 32>), dim3((unsigned)chunks), dim3(kThreads), 0, st, tb, h);
+            else hipLaunchKernelGGL((adamw_kernel<T, 8>), dim3((unsigned)chunks), dim3(kThreads), 0, st, tb, h);
+        };
+        FSC_WITH_DTYPE(dtype, launch);
+        FSC_LAUNCH_CHECK("fsc_adamw_step");
+    }
+    return 0;
+}
+
+}  // extern "C"

@@ -1,0 +1,407 @@
+// Short causal convolution along time, one filter of K <= 8 taps a channel, SiLU behind it (the sequence head's local mixing).
+//   pre[t] = bias + sum_k w[k] xin[t + k],  xin = [K - 1 frames before | x];  y = silu(pre)
+// Bound: HBM (two passes over the frames forward, three backward), K multiply-adds and one exponential a value.  So each thread owns
+// 16 bytes of channels (8 backward in 16 bits) and walks a strip of frames with the filter's window in registers: every frame is read
+// once but for the K - 1 at a strip's ends, neighbouring threads read neighbouring channels.  Frames are taken eight at a time, all
+// their loads issued before the first is used.
+// Backward: the strip recomputes pre (cheaper than keeping it) and runs K - 1 frames past its end; dw / db are summed in registers, over
+// the block's strips through LDS, over blocks by a second launch in a fixed order: equal inputs give equal bits.
+#include <type_traits>
+
+#include "seq.h"
+
+namespace {
+
+using fsc::load_row;
+using fsc::store_row;
+
+constexpr int kThreads = 256;
+
+__device__ __forceinline__ float sigmoid_fast(float v) {
+    return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(v * -1.44269504088896340736f));
+}
+
+struct Plan {
+    int groups;        // of V channels
+    int strip, strips; // frames a thread walks, strips of one sequence
+    int lanes;         // threads along the channel groups (a power of two), kThreads / lanes rows (sequence, strip) a block
+    int rows;          // batch * strips
+    int wide;          // every row of V channels is whole and aligned
+};
+
+__device__ __forceinline__ int frames_of(const fsc_causal_conv_args& a, int n) {
+    if (a.lengths == nullptr) return a.length;
+    const int l = a.lengths[n];
+    return l < 0 ? 0 : l > a.length ? a.length : l;
+}
+
+// Channels c .. c + V - 1 of frame t >= -(K - 1) of sequence n: x, the frames before it, or zeros behind its end.
+template <typename T, int V>
+__device__ __forceinline__ void frame(const fsc_causal_conv_args& a, int n, int c, int t, int len, bool wide, int have, float (&out)[V]) {
+    if (t >= 0 && t < len) {
+        load_row<V>(reinterpret_cast<const T*>(a.x) + n * a.x_batch + t * a.x_time + c, wide, have, out);
+    } else if (t < 0 && a.initial != nullptr) {
+        load_row<V>(reinterpret_cast<const T*>(a.initial) + ((long)n * (a.taps - 1) + a.taps - 1 + t) * a.channels + c, wide, have, out);
+    } else {
+#pragma unroll
+        for (int i = 0; i < V; ++i) out[i] = 0.f;
+    }
+}
+
+template <int K, int V>
+__device__ __forceinline__ void filters(const fsc_causal_conv_args& a, int c, int have, float (&w)[K][V], float (&bias)[V]) {
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+        bias[i] = i < have && a.bias != nullptr ? a.bias[c + i] : 0.f;
+#pragma unroll
+        for (int k = 0; k < K; ++k) w[k][i] = i < have ? a.weight[(long)(c + i) * K + k] : 0.f;
+    }
+}
+
+template <typename T, int K, int V>
+__global__ __launch_bounds__(kThreads) void conv_fwd_kernel(fsc_causal_conv_args a, Plan p) {
+    constexpr int U = 8;
+    const int g = blockIdx.y * p.lanes + (threadIdx.x & (p.lanes - 1));
+    const long row = (long)blockIdx.x * (kThreads / p.lanes) + threadIdx.x / p.lanes;
+    if (g >= p.groups || row >= p.rows) return;
+    const int n = (int)(row / p.strips), s = (int)(row % p.strips), c = g * V;
+    const int have = a.channels - c < V ? a.channels - c : V;
+    const bool wide = p.wide;
+    const int len = frames_of(a, n);
+    if (s == 0 && a.final != nullptr) {
+        for (int j = 0; j < K - 1; ++j) {
+            float v[V];
+            frame<T, V>(a, n, c, len - (K - 1) + j, len, wide, have, v);
+            store_row<V>(reinterpret_cast<T*>(a.final) + ((long)n * (K - 1) + j) * a.channels + c, wide, have, v);
+        }
+    }
+    float w[K][V], bias[V];
+    filters<K, V>(a, c, have, w, bias);
+    const int t0 = s * p.strip, t1 = t0 + p.strip < a.length ? t0 + p.strip : a.length;
+    float x[K - 1 + U][V];
+#pragma unroll
+    for (int j = 0; j < K - 1; ++j) frame<T, V>(a, n, c, t0 - (K - 1) + j, len, wide, have, x[j]);
+    T* out = reinterpret_cast<T*>(a.y) + ((long)n * a.length + t0) * a.channels + c;
+    for (int t = t0; t < t1; t += U) {
+#pragma unroll
+        for (int j = 0; j < U; ++j) frame<T, V>(a, n, c, t + j, len, wide, have, x[K - 1 + j]);
+#pragma unroll
+        for (int j = 0; j < U; ++j) {
+            if (t + j >= t1) break;
+            float y[V];
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+                float v = bias[i];
+#pragma unroll
+                for (int k = 0; k < K; ++k) v = fmaf(w[k][i], x[j + k][i], v);
+                y[i] = t + j < len ? (a.silu ? v * sigmoid_fast(v) : v) : 0.f;
+            }
+            store_row<V>(out, wide, have, y);
+            out += a.channels;
+        }
+#pragma unroll
+        for (int j = 0; j < K - 1; ++j)
+#pragma unroll
+            for (int i = 0; i < V; ++i) x[j][i] = x[U + j][i];
+    }
+}
+
+template <typename T, int K, int V>
+__global__ __launch_bounds__(kThreads) void conv_bwd_kernel(fsc_causal_conv_args a, Plan p) {
+    constexpr int U = 4;
+    __shared__ float red[kThreads][V];
+    const int lane = threadIdx.x & (p.lanes - 1), sub = threadIdx.x / p.lanes, subs = kThreads / p.lanes;
+    const int g = blockIdx.y * p.lanes + lane, c = g * V;
+    const bool mine = g < p.groups;
+    const int have = !mine ? 0 : a.channels - c < V ? a.channels - c : V;
+    const bool wide = p.wide && mine;
+    float w[K][V], bias[V], dw[K][V], db[V];
+    filters<K, V>(a, mine ? c : 0, have, w, bias);
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+        db[i] = 0.f;
+#pragma unroll
+        for (int k = 0; k < K; ++k) dw[k][i] = 0.f;
+    }
+    for (long row = (long)blockIdx.x * subs + sub; mine && row < p.rows; row += (long)gridDim.x * subs) {
+        const int n = (int)(row / p.strips), s = (int)(row % p.strips);
+        const int len = frames_of(a, n);
+        const int t0 = s * p.strip, t1 = t0 + p.strip < a.length ? t0 + p.strip : a.length;
+        float x[K - 1 + U][V], dp[K - 1 + U][V];
+#pragma unroll
+        for (int j = 0; j < K - 1; ++j) {
+            frame<T, V>(a, n, c, t0 - (K - 1) + j, len, wide, have, x[j]);
+#pragma unroll
+            for (int i = 0; i < V; ++i) dp[j][i] = 0.f;
+        }
+        // frame t yields d pre[t]; with it frame t - (K - 1) has its gradient
+        for (int t = t0; t < t1 + K - 1; t += U) {
+            float dy[U][V];
+#pragma unroll
+            for (int j = 0; j < U; ++j) {
+                frame<T, V>(a, n, c, t + j, len, wide, have, x[K - 1 + j]);
+                if (a.dy != nullptr && t + j < len) {
+                    load_row<V>(reinterpret_cast<const T*>(a.dy) + n * a.dy_batch + (t + j) * a.dy_time + c, wide, have, dy[j]);
+                } else {
+#pragma unroll
+                    for (int i = 0; i < V; ++i) dy[j][i] = 0.f;
+                }
+            }
+#pragma unroll
+            for (int j = 0; j < U; ++j) {
+#pragma unroll
+                for (int i = 0; i < V; ++i) {
+                    float grad = dy[j][i];
+                    if (a.silu) {
+                        float v = bias[i];
+#pragma unroll
+                        for (int k = 0; k < K; ++k) v = fmaf(w[k][i], x[j + k][i], v);
+                        const float sig = sigmoid_fast(v);
+                        grad *= sig * fmaf(v, 1.0f - sig, 1.0f);
+                    }
+                    if (t + j >= len) grad = 0.f;
+                    dp[K - 1 + j][i] = grad;
+                    if (t + j < t1) {                              // (the frames past the strip are summed by the next one)
+                        db[i] += grad;
+#pragma unroll
+                        for (int k = 0; k < K; ++k) dw[k][i] = fmaf(grad, x[j + k][i], dw[k][i]);
+                    }
+                }
+                const int at = t + j - (K - 1);
+                if (at >= t1 || (at < t0 && s > 0) || (at < 0 && (a.dinitial == nullptr || at < -(K - 1)))) continue;
+                float dx[V];
+#pragma unroll
+                for (int i = 0; i < V; ++i) {
+                    float v = 0.f;
+#pragma unroll
+                    for (int k = 0; k < K; ++k) v = fmaf(w[K - 1 - k][i], dp[j + k][i], v);
+                    dx[i] = at < len ? v : 0.f;
+                }
+                const int f = at - len + K - 1;                    // among the kept frames
+                if (a.dfinal != nullptr && f >= 0 && f < K - 1) {
+                    float more[V];
+                    load_row<V>(reinterpret_cast<const T*>(a.dfinal) + ((long)n * (K - 1) + f) * a.channels + c, wide, have, more);
+#pragma unroll
+                    for (int i = 0; i < V; ++i) dx[i] += more[i];
+                }
+                T* to = at >= 0 ? reinterpret_cast<T*>(a.dx) + ((long)n * a.length + at) * a.channels + c
+                                : reinterpret_cast<T*>(a.dinitial) + ((long)n * (K - 1) + K - 1 + at) * a.channels + c;
+                store_row<V>(to, wide, have, dx);
+            }
+#pragma unroll
+            for (int j = 0; j < K - 1; ++j)
+#pragma unroll
+                for (int i = 0; i < V; ++i) {
+                    x[j][i] = x[U + j][i];
+                    dp[j][i] = dp[U + j][i];
+                }
+        }
+    }
+    // partial sums of the block: workspace[block][K + 1][groups * V]
+    float* part = reinterpret_cast<float*>(a.workspace) + (long)blockIdx.x * (K + 1) * p.groups * V;
+#pragma unroll
+    for (int k = 0; k <= K; ++k) {
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < V; ++i) red[threadIdx.x][i] = k < K ? dw[k < K ? k : 0][i] : db[i];
+        __syncthreads();
+        if (sub == 0 && mine) {
+            float v[V];
+#pragma unroll
+            for (int i = 0; i < V; ++i) v[i] = red[lane][i];
+            for (int q = 1; q < subs; ++q)
+#pragma unroll
+                for (int i = 0; i < V; ++i) v[i] += red[q * p.lanes + lane][i];
+#pragma unroll
+            for (int i = 0; i < V; ++i) part[(long)k * p.groups * V + c + i] = v[i];
+        }
+    }
+}
+
+// dweight[c, k] / dbias[c]: the blocks' partial sums, 64 columns x 4 interleaved shares of the blocks
+__global__ __launch_bounds__(kThreads) void conv_bwd_finish_kernel(const float* __restrict__ part, int parts, int channels, int padded, int taps,
+                                                                   float* __restrict__ dweight, float* __restrict__ dbias) {
+    __shared__ float red[4][64];
+    const int column = blockIdx.x * 64 + (threadIdx.x & 63), share = threadIdx.x >> 6;
+    const long columns = (long)(taps + 1) * padded;
+    float v0 = 0.f, v1 = 0.f;
+    if (column < columns) {
+        int q = share;
+        for (; q + 4 < parts; q += 8) {
+            v0 += part[q * columns + column];
+            v1 += part[(q + 4) * columns + column];
+        }
+        if (q < parts) v0 += part[q * columns + column];
+    }
+    red[share][threadIdx.x & 63] = v0 + v1;
+    __syncthreads();
+    if (share != 0 || column >= columns) return;
+    const int k = column / padded, c = column % padded;
+    if (c >= channels) return;
+    const float v = (red[0][column & 63] + red[1][column & 63]) + (red[2][column & 63] + red[3][column & 63]);
+    if (k < taps) dweight[(long)c * taps + k] = v;
+    else if (dbias != nullptr) dbias[c] = v;
+}
+
+// One frame: a thread reads its window, computes, and writes the window one frame on.
+template <typename T, int K, int V>
+__global__ __launch_bounds__(kThreads) void conv_step_kernel(fsc_causal_conv_args a, Plan p) {
+    const int g = blockIdx.y * p.lanes + (threadIdx.x & (p.lanes - 1));
+    const long n = (long)blockIdx.x * (kThreads / p.lanes) + threadIdx.x / p.lanes;
+    if (g >= p.groups || n >= a.batch) return;
+    const int c = g * V;
+    const int have = a.channels - c < V ? a.channels - c : V;
+    const bool wide = p.wide;
+    T* window = reinterpret_cast<T*>(const_cast<void*>(a.initial)) + n * (K - 1) * a.channels + c;
+    float x[K][V], w[K][V], bias[V], y[V];
+#pragma unroll
+    for (int k = 0; k < K - 1; ++k) load_row<V>(window + (long)k * a.channels, wide, have, x[k]);
+    load_row<V>(reinterpret_cast<const T*>(a.x) + n * a.x_batch + c, wide, have, x[K - 1]);
+    filters<K, V>(a, c, have, w, bias);
+#pragma unroll
+    for (int k = 0; k < K - 1; ++k) store_row<V>(window + (long)k * a.channels, wide, have, x[k + 1]);
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+        float v = bias[i];
+#pragma unroll
+        for (int k = 0; k < K; ++k) v = fmaf(w[k][i], x[k][i], v);
+        y[i] = a.silu ? v * sigmoid_fast(v) : v;
+    }
+    store_row<V>(reinterpret_cast<T*>(a.y) + n * a.channels + c, wide, have, y);
+}
+
+// Threads wanted in flight: two waves on each of the 1024 SIMDs.  Long strips read fewer frames twice (K - 1 at each end), short ones
+// fill the card.
+constexpr long kWanted = 2 * 1024 * 64;
+
+Plan plan(const fsc_causal_conv_args& a, int v, bool backward) {
+    Plan p{};
+    p.groups = fsc::ceil_div(a.channels, v);
+    const long frames = (long)a.batch * a.length * p.groups;
+    long strip = frames / kWanted / 8 * 8;
+    const long least = backward ? 16 : 8, most = 64;
+    strip = strip < least ? least : strip > most ? most : strip;
+    p.strip = (int)strip;
+    p.strips = a.length > 0 ? fsc::ceil_div(a.length, strip) : 1;
+    p.lanes = 1;
+    while (p.lanes < 64 && p.lanes < p.groups) p.lanes *= 2;
+    p.rows = a.batch * p.strips;
+    const size_t unit = v * fsc::dtype_bytes(a.dtype);
+    p.wide = a.channels % v == 0 && a.x_batch % v == 0 && a.x_time % v == 0 && a.dy_batch % v == 0 && a.dy_time % v == 0 &&
+             fsc::aligned(a.x, unit) && fsc::aligned(a.initial, unit) && fsc::aligned(a.y, unit) && fsc::aligned(a.final, unit) &&
+             fsc::aligned(a.dy, unit) && fsc::aligned(a.dfinal, unit) && fsc::aligned(a.dx, unit) && fsc::aligned(a.dinitial, unit);
+    return p;
+}
+
+constexpr int kBwdV = 4;
+
+// Blocks along the rows of the backward pass: enough for two blocks a CU, and no more partial sums than that.
+int bwd_parts(const Plan& p) {
+    const int across = fsc::ceil_div(p.groups, p.lanes), need = fsc::ceil_div(p.rows, kThreads / p.lanes);
+    const int most = fsc::ceil_div(1024, across);
+    return need < most ? (need > 0 ? need : 1) : most;
+}
+
+const char* bad(const fsc_causal_conv_args* a) {
+    if (a == nullptr) return "null arguments";
+    if (!fsc::dtype_ok(a->dtype)) return "unknown dtype";
+    if (a->taps < 1 || a->taps > 8) return "1 to 8 taps";
+    if (a->batch < 0 || a->length < 0 || a->channels < 0) return "negative size";
+    if ((long)a->batch * (a->length / 8 + 1) > 0x7FFFFFFFL) return "batch * length is too large";
+    if (a->channels > (1 << 23)) return "more than 2^23 channels";
+    if (a->channels > 0 && a->weight == nullptr) return "null weight";
+    return nullptr;
+}
+
+template <typename Launch>
+void with_taps(int taps, Launch launch) {
+    switch (taps) {
+        case 1: launch(std::integral_constant<int, 1>()); break;
+        case 2: launch(std::integral_constant<int, 2>()); break;
+        case 3: launch(std::integral_constant<int, 3>()); break;
+        case 4: launch(std::integral_constant<int, 4>()); break;
+        case 5: launch(std::integral_constant<int, 5>()); break;
+        case 6: launch(std::integral_constant<int, 6>()); break;
+        case 7: launch(std::integral_constant<int, 7>()); break;
+        default: launch(std::integral_constant<int, 8>()); break;
+    }
+}
+
+}  // namespace
+
+extern "C" {
+
+int fsc_causal_conv_fwd(const fsc_causal_conv_args* args_host, fsc_stream_t stream) {
+    const char* why = bad(args_host);
+    FSC_CHECK_ARG(why == nullptr, "fsc_causal_conv_fwd: %s", why);
+    const fsc_causal_conv_args& a = *args_host;
+    if (a.batch == 0 || a.channels == 0 || (a.length == 0 && a.final == nullptr)) return 0;
+    FSC_CHECK_ARG(a.length == 0 || (a.x && a.y), "fsc_causal_conv_fwd: null x or y");
+    auto typed = [&](auto type) {
+        using T = decltype(type);
+        constexpr int V = 16 / sizeof(T);
+        const Plan p = plan(a, V, false);
+        const dim3 grid(fsc::ceil_div(p.rows, kThreads / p.lanes), fsc::ceil_div(p.groups, p.lanes));
+        with_taps(a.taps, [&](auto taps) {
+            hipLaunchKernelGGL((conv_fwd_kernel<T, decltype(taps)::value, V>), grid, dim3(kThreads), 0, fsc::as_stream(stream), a, p);
+        });
+    };
+    FSC_WITH_DTYPE(a.dtype, typed);
+    FSC_LAUNCH_CHECK("fsc_causal_conv_fwd");
+    return 0;
+}
+
+size_t fsc_causal_conv_bwd_workspace_bytes(const fsc_causal_conv_args* args_host) {
+    if (bad(args_host) != nullptr) return 0;
+    const fsc_causal_conv_args& a = *args_host;
+    const Plan p = plan(a, kBwdV, true);
+    return sizeof(float) * (size_t)bwd_parts(p) * (a.taps + 1) * p.groups * kBwdV;
+}
+
+int fsc_causal_conv_bwd(const fsc_causal_conv_args* args_host, fsc_stream_t stream) {
+    const char* why = bad(args_host);
+    FSC_CHECK_ARG(why == nullptr, "fsc_causal_conv_bwd: %s", why);
+    const fsc_causal_conv_args& a = *args_host;
+    if (a.channels == 0) return 0;
+    FSC_CHECK_ARG(a.dweight && a.workspace, "fsc_causal_conv_bwd: null dweight or workspace");
+    FSC_CHECK_ARG(a.batch == 0 || a.length == 0 || (a.x && a.dx), "fsc_causal_conv_bwd: null x or dx");
+    const Plan p = plan(a, kBwdV, true);
+    const int parts = bwd_parts(p);
+    auto typed = [&](auto type) {
+        using T = decltype(type);
+        const dim3 grid(parts, fsc::ceil_div(p.groups, p.lanes));
+        with_taps(a.taps, [&](auto taps) {
+            hipLaunchKernelGGL((conv_bwd_kernel<T, decltype(taps)::value, kBwdV>), grid, dim3(kThreads), 0, fsc::as_stream(stream), a, p);
+        });
+    };
+    FSC_WITH_DTYPE(a.dtype, typed);
+    FSC_LAUNCH_CHECK("fsc_causal_conv_bwd");
+    const int padded = p.groups * kBwdV;
+    hipLaunchKernelGGL(conv_bwd_finish_kernel, dim3(fsc::ceil_div((long)(a.taps + 1) * padded, 64)), dim3(kThreads), 0,
+                       fsc::as_stream(stream), reinterpret_cast<const float*>(a.workspace), parts, a.channels, padded, a.taps, a.dweight,
+                       a.dbias);
+    FSC_LAUNCH_CHECK("fsc_causal_conv_bwd (sums)");
+    return 0;
+}
+
+int fsc_causal_conv_step(const fsc_causal_conv_args* args_host, fsc_stream_t stream) {
+    const char* why = bad(args_host);
+    FSC_CHECK_ARG(why == nullptr, "fsc_causal_conv_step: %s", why);
+    const fsc_causal_conv_args& a = *args_host;
+    if (a.batch == 0 || a.channels == 0) return 0;
+    FSC_CHECK_ARG(a.x && a.y && (a.taps == 1 || a.initial), "fsc_causal_conv_step: null x, y or window");
+    auto typed = [&](auto type) {
+        using T = decltype(type);
+        constexpr int V = 16 / sizeof(T);
+        const Plan p = plan(a, V, false);
+        const dim3 grid(fsc::ceil_div(a.batch, kThreads / p.lanes), fsc::ceil_div(p.groups, p.lanes));
+        with_taps(a.taps, [&](auto taps) {
+            hipLaunchKernelGGL((conv_step_kernel<T, decltype(taps)::value, V>), grid, dim3(kThreads), 0, fsc::as_stream(stream), a, p);
+        });
+    };
+    FSC_WITH_DTYPE(a.dtype, typed);
+    FSC_LAUNCH_CHECK("fsc_causal_conv_step");
+    return 0;
+}
+
+}  // extern "C"

@@ -1,0 +1,440 @@
+// Selective scan, backward (scan.h says how the work is split).  With dyy = dy silu(z), e_t = exp(delta_t A) and G_t = dL/dh_t:
+//   G_t = C_t dyy_t + e_{t+1} G_{t+1}        dC_t = sum_d h_t dyy_t           dB_t = sum_d G_t delta_t u_t
+//   du = delta sum_s G B + D dyy              d delta = sum_s G (A e h_{t-1} + u B)      dA = sum_{n,t} G delta e h_{t-1}
+//   dz = dy (C.h + D u) silu'(z)              ddt = d delta sigmoid(dt + bias)           dD = sum dyy u,  dh_{-1} = e_0 G_0
+// A tile of 16 frames starts from the state that the forward kept there: e and h_{t-1} of its frames are formed once, forwards, and stay in
+// registers (2 x 16 x NS) for the way back, so an element costs one exponential and some fifteen multiply-adds.
+// The sums over the channels (dB, dC) take the wave's channels by lane exchanges that halve the number of values at each turn, the
+// four waves through LDS, the blocks in a second launch; dA, dD and d dt_bias are summed in registers over time and by the second launch
+// over sequences and segments.  No atomics: equal inputs give equal bits.
+#include <type_traits>
+
+#include "scan.h"
+
+namespace {
+
+using namespace fsc;
+
+// The workspace: segments' ends and their deltas (one segment: none), partial sums over channel blocks and over (sequence, segment).
+struct Carve {
+    size_t ends, end_deltas, rows, sums, bytes;      // offsets in floats
+    Carve(const fsc_selective_scan_args& a, const ScanPlan& p) {
+        const size_t many = (size_t)a.batch * p.segments, channels = p.padded_channels(), sp = p.padded_states();
+        ends = 0;
+        end_deltas = p.segments > 1 ? many * channels * sp : 0;
+        rows = end_deltas + (p.segments > 1 ? many * channels : 0);
+        sums = rows + (size_t)a.batch * p.blocks * p.tiles * kTile * 2 * sp;
+        bytes = sizeof(float) * (sums + many * channels * (sp + 2));
+    }
+};
+
+// A segment's gradient of the state in front of it, from zero behind it: G as in the main pass, nothing else.
+template <typename T, int L, int NS>
+__global__ __launch_bounds__(256) void scan_bwd_ends_kernel(fsc_selective_scan_args a, ScanPlan p, float* ends, float* end_deltas) {
+    using Place = ScanPlace<L, NS>;
+    constexpr int CB = Place::CB, E = Place::E, SP = Place::SP, ROWS = Place::ROWS;
+    __shared__ __align__(16) float s_delta[CB][kPad], s_dyy[CB][kPad], s_c[kTile][SP];
+    const Place w(a, p);
+    if (w.segment == 0) return;
+    const int len = scan_frames(a, w.n);
+    const int first = w.segment * p.segment_tiles;
+    const int last = first + p.segment_tiles < p.tiles ? first + p.segment_tiles : p.tiles;
+    float a2[NS], e[NS] = {}, sum = 0.f;
+    scan_rates(a, w, a2);
+    float bias[E];
+#pragma unroll
+    for (int i = 0; i < E; ++i) bias[i] = a.dt_bias != nullptr && i < w.he ? a.dt_bias[w.c0 + w.ce + i] : 0.f;
+    const bool wide = p.wide && w.he == E;
+    const long c = w.c0 + w.ce;
+    const int work_end = tiles_with(len) < last ? tiles_with(len) : last;
+    for (int tile = work_end - 1; tile >= first; --tile) {
+        const int t = tile * kTile + w.te, he = t < len ? w.he : 0;
+        const bool go = wide && t < len;
+        float dt[E], z[E], dy[E];
+        load_row<E>(reinterpret_cast<const T*>(a.dt) + w.n * a.dt_batch + t * a.dt_time + c, go, he, dt);
+        load_row<E>(reinterpret_cast<const T*>(a.dy) + w.n * a.dy_batch + t * a.dy_time + c, go && a.dy != nullptr, a.dy != nullptr ? he : 0, dy);
+        if (a.z != nullptr) load_row<E>(reinterpret_cast<const T*>(a.z) + w.n * a.z_batch + t * a.z_time + c, go, he, z);
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < E; ++i) {
+            const float raw = dt[i] + bias[i];
+            s_delta[w.ce + i][w.te] = t < len ? (a.softplus ? softplus_fast(raw) : raw) : 0.f;
+            s_dyy[w.ce + i][w.te] = a.z != nullptr ? dy[i] * (z[i] * sigmoid_fast(z[i])) : dy[i];
+        }
+#pragma unroll
+        for (int j = 0; j < ROWS; ++j)
+            if (w.bc_mine(j)) {
+                const int tr = tile * kTile + w.bc_row(j), s = w.bc_state(j);
+                s_c[w.bc_row(j)][s] =
+                    tr < len && s < a.states ? (float)reinterpret_cast<const T*>(a.c)[w.n * a.c_batch + tr * a.c_time + w.group * a.c_group + s] : 0.f;
+            }
+        __syncthreads();
+#pragma unroll
+        for (int q = kTile / 4 - 1; q >= 0; --q) {
+            float dl[4], dyy[4];
+            load_row<4>(&s_delta[w.ch][4 * q], true, 4, dl);
+            load_row<4>(&s_dyy[w.ch][4 * q], true, 4, dyy);
+#pragma unroll
+            for (int j = 3; j >= 0; --j) {
+                float cc[NS];
+                load_row<NS>(&s_c[4 * q + j][w.sg * NS], true, NS, cc);
+#pragma unroll
+                for (int i = 0; i < NS; ++i) e[i] = __builtin_amdgcn_exp2f(dl[j] * a2[i]) * fmaf(cc[i], dyy[j], e[i]);
+                sum += dl[j];
+            }
+        }
+    }
+    store_row<NS>(ends + w.end(p, w.segment), true, NS, e);
+    if (w.sg == 0) end_deltas[w.end_delta(p, w.segment)] = sum;
+}
+
+// The sums of v[0 .. 2 NS) over the channels of a wave (lanes that differ above the L lanes of one channel).  On return v[0 .. kept)
+// hold the sums of the values first .. first + kept - 1.
+template <int L, int NS>
+__device__ __forceinline__ void channel_sums(float (&v)[2 * NS], int lane) {
+    constexpr int N = 2 * NS;
+#pragma unroll
+    for (int i = 0; i < N / 2; ++i) {
+        swap32(v[i], v[i + N / 2]);
+        v[i] += v[i + N / 2];
+    }
+    if constexpr (N >= 4) {
+#pragma unroll
+        for (int i = 0; i < N / 4; ++i) {
+            swap16(v[i], v[i + N / 4]);
+            v[i] += v[i + N / 4];
+        }
+    } else {
+        float other = v[0];
+        swap16(v[0], other);
+        v[0] += other;
+    }
+    constexpr int kept = N >= 4 ? N / 4 : 1;
+#pragma unroll
+    for (int i = 0; i < kept; ++i) {
+        if constexpr (L <= 8) v[i] += dpp<0x128>(v[i]);
+        if constexpr (L <= 4) v[i] += dpp<0x124>(v[i]);
+    }
+}
+
+template <typename T, int L, int NS>
+__global__ __launch_bounds__(256, 2) void scan_bwd_kernel(fsc_selective_scan_args a, ScanPlan p, Carve at) {
+    using Place = ScanPlace<L, NS>;
+    constexpr int CB = Place::CB, E = Place::E, SP = Place::SP, ROWS = Place::ROWS;
+    __shared__ __align__(16) float s_delta[CB][kPad], s_du[CB][kPad], s_dyy[CB][kPad], s_yh[CB][kPad];
+    __shared__ __align__(16) float s_b[kTile][SP], s_c[kTile][SP];
+    __shared__ __align__(16) float s_red[kTile][4][2][SP];
+    float* ws = reinterpret_cast<float*>(a.workspace);
+    const Place w(a, p);
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int len = scan_frames(a, w.n);
+    const int first = w.segment * p.segment_tiles;
+    const int last = first + p.segment_tiles < p.tiles ? first + p.segment_tiles : p.tiles;
+
+    float a2[NS], e[NS], da[NS] = {};              // e: exp(delta_{t+1} A) G_{t+1}, what reaches h_t from behind
+    scan_rates(a, w, a2);
+    scan_state(a, w, a.dfinal, e);
+    for (int q = p.segments - 1; q > w.segment; --q) {
+        const float ds = ws[at.end_deltas + w.end_delta(p, q)];
+        float more[NS];
+        load_row<NS>(ws + at.ends + w.end(p, q), true, NS, more);
+#pragma unroll
+        for (int i = 0; i < NS; ++i) e[i] = fmaf(__builtin_amdgcn_exp2f(a2[i] * ds), e[i], more[i]);
+    }
+    float bias[E], skip[E], dskip[E] = {}, dbias[E] = {};
+#pragma unroll
+    for (int i = 0; i < E; ++i) {
+        bias[i] = a.dt_bias != nullptr && i < w.he ? a.dt_bias[w.c0 + w.ce + i] : 0.f;
+        skip[i] = a.d != nullptr && i < w.he ? a.d[w.c0 + w.ce + i] : 0.f;
+    }
+    const bool wide = p.wide && w.he == E;
+    const long c = w.c0 + w.ce;
+    float u_next[E], dt_next[E], z_next[E], dy_next[E], b_next[ROWS], c_next[ROWS], h_next[NS];
+    auto fetch = [&](int tile) {
+        const int t = tile * kTile + w.te;
+        const int he = t < len ? w.he : 0;
+        const bool go = wide && t < len;
+        load_row<E>(reinterpret_cast<const T*>(a.u) + w.n * a.u_batch + t * a.u_time + c, go, he, u_next);
+        load_row<E>(reinterpret_cast<const T*>(a.dt) + w.n * a.dt_batch + t * a.dt_time + c, go, he, dt_next);
+        if (a.z != nullptr) load_row<E>(reinterpret_cast<const T*>(a.z) + w.n * a.z_batch + t * a.z_time + c, go, he, z_next);
+        load_row<E>(reinterpret_cast<const T*>(a.dy) + w.n * a.dy_batch + t * a.dy_time + c, go && a.dy != nullptr, a.dy != nullptr ? he : 0, dy_next);
+#pragma unroll
+        for (int j = 0; j < ROWS; ++j) {
+            const int tr = tile * kTile + w.bc_row(j), s = w.bc_state(j);
+            const bool there = w.bc_mine(j) && tr < len && s < a.states;
+            b_next[j] = there ? (float)reinterpret_cast<const T*>(a.b)[w.n * a.b_batch + tr * a.b_time + w.group * a.b_group + s] : 0.f;
+            c_next[j] = there ? (float)reinterpret_cast<const T*>(a.c)[w.n * a.c_batch + tr * a.c_time + w.group * a.c_group + s] : 0.f;
+        }
+        load_row<NS>(a.checkpoints + w.kept(p, tile), true, NS, h_next);
+    };
+    const int work_end = tiles_with(len) < last ? tiles_with(len) : last;      // tiles behind it hold no frame
+    for (int tile = work_end > first ? work_end : first; tile < last; ++tile) {
+        const int t = tile * kTile + w.te;
+        float zero[E] = {};
+        if (t < a.length) {
+            const long o = ((long)w.n * a.length + t) * a.channels + c;
+            store_row<E>(reinterpret_cast<T*>(a.du) + o, wide, w.he, zero);
+            store_row<E>(reinterpret_cast<T*>(a.ddt) + o, wide, w.he, zero);
+            if (a.z != nullptr) store_row<E>(reinterpret_cast<T*>(a.dz) + o, wide, w.he, zero);
+        }
+        for (int j = threadIdx.x; j < kTile * 2 * SP; j += 256)
+            ws[at.rows + (((long)w.n * p.blocks + w.block) * p.tiles + tile) * (kTile * 2 * SP) + j] = 0.f;
+    }
+    if (first < work_end) fetch(work_end - 1);
+    for (int tile = work_end - 1; tile >= first; --tile) {
+        const int t = tile * kTile + w.te;
+        float u[E], delta[E], sig[E], gz[E], dyy[E], h[NS], hp[kTile][NS], ex[kTile][NS];
+#pragma unroll
+        for (int i = 0; i < E; ++i) {
+            u[i] = u_next[i];
+            const float raw = dt_next[i] + bias[i];
+            delta[i] = t < len ? (a.softplus ? softplus_fast(raw) : raw) : 0.f;
+            sig[i] = t < len ? (a.softplus ? sigmoid_fast(raw) : 1.0f) : 0.f;
+            dyy[i] = dy_next[i];
+            gz[i] = 0.f;
+            if (a.z != nullptr) {
+                const float s = sigmoid_fast(z_next[i]);
+                gz[i] = dy_next[i] * (s * fmaf(z_next[i], 1.0f - s, 1.0f));
+                dyy[i] = dy_next[i] * (z_next[i] * s);
+            }
+            s_delta[w.ce + i][w.te] = delta[i];
+            s_du[w.ce + i][w.te] = delta[i] * u[i];
+            s_dyy[w.ce + i][w.te] = dyy[i];
+        }
+#pragma unroll
+        for (int j = 0; j < ROWS; ++j)
+            if (w.bc_mine(j)) {
+                s_b[w.bc_row(j)][w.bc_state(j)] = b_next[j];
+                s_c[w.bc_row(j)][w.bc_state(j)] = c_next[j];
+            }
+#pragma unroll
+        for (int i = 0; i < NS; ++i) h[i] = h_next[i];
+        __syncthreads();
+        if (tile > first) fetch(tile - 1);
+#pragma unroll
+        for (int q = 0; q < kTile / 4; ++q) {
+            float dl[4], du[4], y[4];
+            load_row<4>(&s_delta[w.ch][4 * q], true, 4, dl);
+            load_row<4>(&s_du[w.ch][4 * q], true, 4, du);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                float b[NS], cc[NS], v = 0.f;
+                load_row<NS>(&s_b[4 * q + j][w.sg * NS], true, NS, b);
+                load_row<NS>(&s_c[4 * q + j][w.sg * NS], true, NS, cc);
+#pragma unroll
+                for (int i = 0; i < NS; ++i) {
+                    ex[4 * q + j][i] = __builtin_amdgcn_exp2f(dl[j] * a2[i]);
+                    hp[4 * q + j][i] = h[i];
+                    h[i] = fmaf(ex[4 * q + j][i], h[i], du[j] * b[i]);
+                    v = fmaf(cc[i], h[i], v);
+                }
+                y[j] = group_sum<L>(v);
+            }
+            const int k = w.sg & 3;
+            const float mine = k == 0 ? y[0] : k == 1 ? y[1] : k == 2 ? y[2] : y[3];
+            if (w.sg < 4) s_yh[w.ch][4 * q + k] = mine;
+        }
+#pragma unroll
+        for (int q = kTile / 4 - 1; q >= 0; --q) {
+            float dl[4], du[4], dyy4[4], gb4[4], ga4[4];
+            load_row<4>(&s_delta[w.ch][4 * q], true, 4, dl);
+            load_row<4>(&s_du[w.ch][4 * q], true, 4, du);
+            load_row<4>(&s_dyy[w.ch][4 * q], true, 4, dyy4);
+#pragma unroll
+            for (int j = 3; j >= 0; --j) {
+                const int k = 4 * q + j;
+                float b[NS], cc[NS], v[2 * NS], gb = 0.f, ga = 0.f;
+                load_row<NS>(&s_b[k][w.sg * NS], true, NS, b);
+                load_row<NS>(&s_c[k][w.sg * NS], true, NS, cc);
+#pragma unroll
+                for (int i = 0; i < NS; ++i) {
+                    const float g = fmaf(cc[i], dyy4[j], e[i]);
+                    v[i] = g * du[j];
+                    v[NS + i] = h[i] * dyy4[j];
+                    gb = fmaf(g, b[i], gb);
+                    const float gx = g * (ex[k][i] * hp[k][i]);
+                    da[i] = fmaf(gx, dl[j], da[i]);
+                    ga = fmaf(gx, a2[i], ga);
+                    e[i] = ex[k][i] * g;
+                    h[i] = hp[k][i];
+                }
+                gb4[j] = group_sum<L>(gb);
+                ga4[j] = group_sum<L>(ga);
+                channel_sums<L, NS>(v, lane);
+                // upper half: dC, lower half: dB; even rows of 16 lanes: the first half of the states, odd rows: the second
+                constexpr int kept = NS >= 2 ? NS / 2 : 1;
+                const int half = lane >> 5, row = (lane >> 4) & 1;
+                if ((lane & 15) < L && (NS >= 2 || row == 0)) {
+                    const int s = w.sg * NS + (NS >= 2 ? row * kept : 0);
+#pragma unroll
+                    for (int i = 0; i < kept; ++i) s_red[k][wave][half][s + i] = v[i];
+                }
+            }
+            // (the four frames' delta and delta u have been read by all lanes of this channel: their places take the sums)
+            const int k = w.sg & 3;
+            const float mine_b = k == 0 ? gb4[0] : k == 1 ? gb4[1] : k == 2 ? gb4[2] : gb4[3];
+            const float mine_a = k == 0 ? ga4[0] : k == 1 ? ga4[1] : k == 2 ? ga4[2] : ga4[3];
+            if (w.sg < 4) {
+                s_du[w.ch][4 * q + k] = mine_b;
+                s_delta[w.ch][4 * q + k] = mine_a;
+            }
+        }
+        __syncthreads();
+        for (int j = threadIdx.x; j < kTile * 2 * SP; j += 256) {
+            const int k = j / (2 * SP), rest = j % (2 * SP);
+            const float* r = &s_red[k][0][0][rest];
+            ws[at.rows + (((long)w.n * p.blocks + w.block) * p.tiles + tile) * (kTile * 2 * SP) + j] =
+                (r[0] + r[2 * SP]) + (r[4 * SP] + r[6 * SP]);
+        }
+        if (t < a.length) {
+            float du_out[E], ddt_out[E], dz_out[E];
+#pragma unroll
+            for (int i = 0; i < E; ++i) {
+                const float gb = s_du[w.ce + i][w.te], ga = s_delta[w.ce + i][w.te] * kLn2;
+                du_out[i] = fmaf(delta[i], gb, skip[i] * dyy[i]);
+                ddt_out[i] = fmaf(u[i], gb, ga) * sig[i];
+                dz_out[i] = gz[i] * fmaf(skip[i], u[i], s_yh[w.ce + i][w.te]);
+                if (t >= len) du_out[i] = ddt_out[i] = dz_out[i] = 0.f;
+                dskip[i] = fmaf(dyy[i], u[i], dskip[i]);
+                dbias[i] += ddt_out[i];
+            }
+            const long o = ((long)w.n * a.length + t) * a.channels + c;
+            store_row<E>(reinterpret_cast<T*>(a.du) + o, wide, w.he, du_out);
+            store_row<E>(reinterpret_cast<T*>(a.ddt) + o, wide, w.he, ddt_out);
+            if (a.z != nullptr) store_row<E>(reinterpret_cast<T*>(a.dz) + o, wide, w.he, dz_out);
+        }
+        __syncthreads();
+    }
+    if (a.dinitial != nullptr && w.segment == 0 && w.real) {
+#pragma unroll
+        for (int i = 0; i < NS; ++i) {
+            const int s = w.sg * NS + i;
+            if (s < a.states) a.dinitial[((long)w.n * a.channels + w.channel) * a.states + s] = e[i];
+        }
+    }
+    // this (sequence, segment)'s share of the parameters' gradients: [dA: channels x SP | dD | d dt_bias]
+    const long channels = p.padded_channels();
+    float* mine = ws + at.sums + ((long)w.n * p.segments + w.segment) * channels * (SP + 2);
+    store_row<NS>(mine + ((long)w.block * 256 + threadIdx.x) * NS, true, NS, da);
+#pragma unroll
+    for (int i = 0; i < E; ++i) {
+        s_dyy[w.ce + i][w.te] = dskip[i];
+        s_yh[w.ce + i][w.te] = dbias[i];
+    }
+    __syncthreads();
+    if (threadIdx.x < CB) {
+        float sd = 0.f, sb = 0.f;
+#pragma unroll
+        for (int k = 0; k < kTile; ++k) {
+            sd += s_dyy[threadIdx.x][k];
+            sb += s_yh[threadIdx.x][k];
+        }
+        mine[channels * SP + w.block * CB + threadIdx.x] = sd;
+        mine[channels * (SP + 1) + w.block * CB + threadIdx.x] = sb;
+    }
+}
+
+// Joins the partial sums: the first `row_blocks` workgroups dB / dC over the channel blocks of a group, the others (64 columns x 4
+// interleaved shares) the parameters' over sequences and segments.
+template <typename T>
+__global__ __launch_bounds__(256) void scan_bwd_finish_kernel(fsc_selective_scan_args a, ScanPlan p, Carve at, long row_blocks) {
+    const float* ws = reinterpret_cast<const float*>(a.workspace);
+    const int sp = p.padded_states();
+    if (blockIdx.x < row_blocks) {
+        const long i = (long)blockIdx.x * 256 + threadIdx.x;         // (sequence, frame, group, state)
+        if (i >= (long)a.batch * a.length * a.groups * a.states) return;
+        const int s = (int)(i % a.states);
+        const long r = i / a.states;
+        const int g = (int)(r % a.groups);
+        const long f = r / a.groups;
+        const int n = (int)(f / a.length), t = (int)(f % a.length);
+        const long stride = (long)p.tiles * kTile * 2 * sp;
+        const float* from = ws + at.rows + ((long)n * p.blocks + (long)g * p.group_blocks) * stride + (long)t * 2 * sp + s;
+        float db = 0.f, dc = 0.f;
+        for (int q = 0; q < p.group_blocks; ++q) {
+            db += from[q * stride];
+            dc += from[q * stride + sp];
+        }
+        reinterpret_cast<T*>(a.db)[i] = (T)db;
+        reinterpret_cast<T*>(a.dc)[i] = (T)dc;
+        return;
+    }
+    __shared__ float red[4][64];
+    const long channels = p.padded_channels(), columns = channels * (sp + 2);
+    const long column = ((long)blockIdx.x - row_blocks) * 64 + (threadIdx.x & 63);
+    const int share = threadIdx.x >> 6, count = a.batch * p.segments;
+    float v0 = 0.f, v1 = 0.f;
+    if (column < columns) {
+        const float* from = ws + at.sums + column;
+        int q = share;
+        for (; q + 4 < count; q += 8) {
+            v0 += from[q * columns];
+            v1 += from[(q + 4) * columns];
+        }
+        if (q < count) v0 += from[q * columns];
+    }
+    red[share][threadIdx.x & 63] = v0 + v1;
+    __syncthreads();
+    if (share != 0 || column >= columns) return;
+    const int k = threadIdx.x & 63;
+    const float v = (red[0][k] + red[1][k]) + (red[2][k] + red[3][k]);
+    const int cb = p.channels_block;
+    const long slot = column < channels * sp ? column / sp : (column - channels * sp) % channels;      // padded channel
+    const int block = (int)(slot / cb), in_group = (block % p.group_blocks) * cb + (int)(slot % cb);
+    if (in_group >= p.group_channels) return;
+    const long c = (long)(block / p.group_blocks) * p.group_channels + in_group;
+    if (column < channels * sp) {
+        const int s = (int)(column % sp);
+        if (s < a.states) a.da_log[c * a.states + s] = -expf(a.a_log[c * a.states + s]) * v;           // dA / d a_log = A
+    } else if (column < channels * (sp + 1)) {
+        if (a.dd != nullptr) a.dd[c] = v;
+    } else if (a.ddt_bias != nullptr) {
+        a.ddt_bias[c] = v;
+    }
+}
+
+}  // namespace
+
+extern "C" {
+
+size_t fsc_selective_scan_workspace_bytes(const fsc_selective_scan_args* args_host, int backward) {
+    if (scan_bad(args_host) != nullptr) return 0;
+    const ScanPlan p = scan_plan(*args_host);
+    const Carve at(*args_host, p);
+    return backward ? at.bytes : sizeof(float) * at.rows;
+}
+
+int fsc_selective_scan_bwd(const fsc_selective_scan_args* args_host, fsc_stream_t stream) {
+    const char* why = scan_bad(args_host);
+    FSC_CHECK_ARG(why == nullptr, "fsc_selective_scan_bwd: %s", why);
+    const fsc_selective_scan_args& a = *args_host;
+    if (a.channels == 0) return 0;
+    const ScanPlan p = scan_plan(a);
+    const Carve at(a, p);
+    FSC_CHECK_ARG(a.da_log && (a.workspace || at.bytes == 0), "fsc_selective_scan_bwd: null da_log or workspace");
+    FSC_CHECK_ARG(a.batch == 0 || a.length == 0 ||
+                      (a.u && a.dt && a.b && a.c && a.checkpoints && a.du && a.ddt && a.db && a.dc && (a.z == nullptr || a.dz)),
+                  "fsc_selective_scan_bwd: null input or gradient");
+    float* ws = reinterpret_cast<float*>(a.workspace);
+    const dim3 grid((unsigned)((long)a.batch * p.blocks * p.segments));
+    const long rows = ((long)a.batch * a.length * a.groups * a.states + 255) / 256;
+    const long columns = (p.padded_channels() * (p.padded_states() + 2) + 63) / 64;
+    FSC_CHECK_ARG(rows + columns < 0x7FFFFFFFL, "fsc_selective_scan_bwd: too large");
+    auto typed = [&](auto type) {
+        using T = decltype(type);
+        if (a.batch > 0)
+            with_scan_shape(p, [&](auto lanes, auto per) {
+                constexpr int L = decltype(lanes)::value, NS = decltype(per)::value;
+                if (p.segments > 1)
+                    hipLaunchKernelGGL((scan_bwd_ends_kernel<T, L, NS>), grid, dim3(256), 0, as_stream(stream), a, p, ws + at.ends,
+                                       ws + at.end_deltas);
+                hipLaunchKernelGGL((scan_bwd_kernel<T, L, NS>), grid, dim3(256), 0, as_stream(stream), a, p, at);
+            });
+        hipLaunchKernelGGL((scan_bwd_finish_kernel<T>), dim3((unsigned)(rows + columns)), dim3(256), 0, as_stream(stream), a, p, at, rows);
+    };
+    FSC_WITH_DTYPE(a.dtype, typed);
+    FSC_LAUNCH_CHECK("fsc_selective_scan_bwd");
+    return 0;
+}
+
+}  // extern "C"

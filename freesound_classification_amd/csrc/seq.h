@@ -1,0 +1,96 @@
+// What the sequence kernels and the decoupled optimizer share: activations in three types, reductions over neighbouring lanes.
+#pragma once
+#include "common.h"
+
+namespace fsc {
+
+typedef __bf16 bf16_t;
+typedef _Float16 f16_t;
+
+// V consecutive values as one load or store (the caller has checked that the address is a multiple of their size)
+template <typename T, int V>
+struct alignas(sizeof(T) * V) Pack {
+    T v[V];
+};
+
+// V consecutive values at `p` as floats: one wide load where `wide`, else one by one and only the first `have` (the others are 0).
+template <int V, typename T>
+__device__ __forceinline__ void load_row(const T* p, bool wide, int have, float (&out)[V]) {
+    if (wide) {
+        const Pack<T, V> w = *reinterpret_cast<const Pack<T, V>*>(p);
+#pragma unroll
+        for (int i = 0; i < V; ++i) out[i] = (float)w.v[i];
+    } else {
+#pragma unroll
+        for (int i = 0; i < V; ++i) out[i] = i < have ? (float)p[i] : 0.f;
+    }
+}
+template <int V, typename T>
+__device__ __forceinline__ void store_row(T* p, bool wide, int have, const float (&in)[V]) {
+    if (wide) {
+        Pack<T, V> w;
+#pragma unroll
+        for (int i = 0; i < V; ++i) w.v[i] = (T)in[i];
+        *reinterpret_cast<Pack<T, V>*>(p) = w;
+    } else {
+#pragma unroll
+        for (int i = 0; i < V; ++i)
+            if (i < have) p[i] = (T)in[i];
+    }
+}
+
+// A neighbour's value within a row of 16 lanes, in the adder's own operand fetch.  CTRL: 0xB1 lane ^ 1, 0x4E lane ^ 2, 0x141 mirrored
+// within 8 (with equal quads: lane ^ 4), 0x140 mirrored within 16 (with equal eights: lane ^ 8), 0x124 / 0x128 turned by 4 / 8 lanes.
+template <int CTRL>
+__device__ __forceinline__ float dpp(float v) {
+    return __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, v), CTRL, 0xf, 0xf, true));
+}
+
+// The sum over aligned groups of L <= 16 lanes, in every lane of the group.
+template <int L>
+__device__ __forceinline__ float group_sum(float v) {
+    if constexpr (L >= 2) v += dpp<0xB1>(v);
+    if constexpr (L >= 4) v += dpp<0x4E>(v);
+    if constexpr (L >= 8) v += dpp<0x141>(v);
+    if constexpr (L >= 16) v += dpp<0x140>(v);
+    return v;
+}
+
+// Lanes 32..63 of `a` change places with lanes 0..31 of `b` (swap32), the odd rows of 16 of `a` with the even rows of `b` (swap16):
+// a + b is then the halfway sum of both, `a`'s in the lower half or the even rows, `b`'s in the others.
+__device__ __forceinline__ void swap32(float& a, float& b) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(unsigned, a), __builtin_bit_cast(unsigned, b), false, false);
+    const unsigned first = r[0], second = r[1];      // (out of the vector first: a bit cast of its element reads element 0)
+    a = __builtin_bit_cast(float, first);
+    b = __builtin_bit_cast(float, second);
+}
+__device__ __forceinline__ void swap16(float& a, float& b) {
+    const auto r = __builtin_amdgcn_permlane16_swap(__builtin_bit_cast(unsigned, a), __builtin_bit_cast(unsigned, b), false, false);
+    const unsigned first = r[0], second = r[1];      // (out of the vector first: a bit cast of its element reads element 0)
+    a = __builtin_bit_cast(float, first);
+    b = __builtin_bit_cast(float, second);
+}
+
+// The largest value of the wave, in every lane; no value is NaN.
+__device__ __forceinline__ float wave_top(float v) {
+    v = fmaxf(v, dpp<0xB1>(v));
+    v = fmaxf(v, dpp<0x4E>(v));
+    v = fmaxf(v, dpp<0x141>(v));
+    v = fmaxf(v, dpp<0x140>(v));
+    float w = v;
+    swap16(v, w);
+    v = w = fmaxf(v, w);
+    swap32(v, w);
+    return fmaxf(v, w);
+}
+
+inline size_t dtype_bytes(int dtype) { return dtype == FSC_DTYPE_F32 ? 4 : 2; }
+inline bool dtype_ok(int dtype) { return dtype == FSC_DTYPE_F32 || dtype == FSC_DTYPE_BF16 || dtype == FSC_DTYPE_F16; }
+// whether `bytes`-wide accesses at p + multiples of `strides` elements stay aligned
+inline bool aligned(const void* p, size_t bytes) { return ((uintptr_t)p & (bytes - 1)) == 0; }
+
+}  // namespace fsc
+
+// `run(T())` with the activation type that `dtype` names
+#define FSC_WITH_DTYPE(dtype, run)                                                                                              \
+    ((dtype) == FSC_DTYPE_F32 ? run(float()) : (dtype) == FSC_DTYPE_BF16 ? run(fsc::bf16_t()) : run(fsc::f16_t()))

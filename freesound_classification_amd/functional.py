@@ -15,6 +15,7 @@ import torch
 
 from . import _lib
 from ._lib import ConvDesc, call, ptr, stream_ptr
+from .sequence import causal_conv, causal_conv_step, selective_scan, selective_scan_step  # noqa: F401  (public here)
 
 BN_EPS = 1e-5
 LOG_EPS = 1e-4
@@ -1689,6 +1690,93 @@ def rnn_head(out, rnn):
     ln, gru = rnn[0], rnn[1]
     return RnnHeadFn.apply(out, ln.eps, ln.weight, ln.bias, gru.weight_ih_l0, gru.weight_hh_l0, gru.bias_ih_l0, gru.bias_hh_l0,
                            gru.weight_ih_l0_reverse, gru.weight_hh_l0_reverse, gru.bias_ih_l0_reverse, gru.bias_hh_l0_reverse)
+
+
+# ------------------------------------------------------------------------------ state-space aggregation head
+class FrameNormFn(torch.autograd.Function):
+    """Mean over frequency and LayerNorm((C,)) of each frame: (N, C, H, W) -> (N, W, C), as in RnnHeadFn."""
+
+    @staticmethod
+    def forward(ctx, out, eps, weight, bias):
+        out = out.contiguous()
+        n, c, h, w = out.shape
+        xm = _empty((n, w, c), out)
+        call("fsc_freq_mean_fwd", ptr(out), ptr(xm), n, c, h, w, stream_ptr())
+        xl = torch.empty_like(xm)
+        mean, rstd = _empty((n * w,), out), _empty((n * w,), out)
+        call("fsc_layernorm_fwd", ptr(xm), ptr(weight), ptr(bias), float(eps), ptr(xl), ptr(mean), ptr(rstd), n * w, c, stream_ptr())
+        ctx.save_for_backward(xm, mean, rstd, weight)
+        ctx.shape = (n, c, h, w)
+        return xl
+
+    @staticmethod
+    def backward(ctx, dxl):
+        xm, mean, rstd, weight = ctx.saved_tensors
+        n, c, h, w = ctx.shape
+        dxm = torch.empty_like(xm)
+        dw, db = _empty((c,), xm), _empty((c,), xm)
+        call("fsc_layernorm_bwd", ptr(dxl.contiguous()), ptr(xm), ptr(mean), ptr(rstd), ptr(weight), ptr(dxm), ptr(dw), ptr(db), n * w, c,
+             stream_ptr())
+        dout = None
+        if ctx.needs_input_grad[0]:
+            dout = _empty((n, c, h, w), xm)
+            call("fsc_freq_mean_bwd", ptr(dxm), ptr(dout), n, c, h, w, stream_ptr())
+        return dout, None, dw, db
+
+
+class FrameMeanFn(torch.autograd.Function):
+    """(N, W, D) -> (N, D): the mean over the frames (the frequency mean's kernels with the frames as rows)."""
+
+    @staticmethod
+    def forward(ctx, y):
+        y = y.contiguous()
+        n, w, d = y.shape
+        out = _empty((n, d), y)
+        call("fsc_freq_mean_fwd", ptr(y), ptr(out), n, 1, w, d, stream_ptr())
+        ctx.shape = (n, w, d)
+        return out
+
+    @staticmethod
+    def backward(ctx, dout):
+        n, w, d = ctx.shape
+        dy = _empty((n, w, d), dout)
+        call("fsc_freq_mean_bwd", ptr(dout.contiguous()), ptr(dy), n, 1, w, d, stream_ptr())
+        return dy
+
+
+class SplitColsFn(torch.autograd.Function):
+    """Contiguous column pieces of a (rows, sum widths) projection; their gradients side by side on the way back."""
+
+    @staticmethod
+    def forward(ctx, full, widths):
+        full = full.contiguous()
+        pieces = [_empty((full.shape[0], w), full) for w in widths]
+        _cat_cols(pieces, widths, full.shape[0], full, 1)
+        ctx.widths = widths
+        return tuple(pieces)
+
+    @staticmethod
+    def backward(ctx, *grads):
+        grads = [g.contiguous() for g in grads]
+        full = _empty((grads[0].shape[0], sum(ctx.widths)), grads[0])
+        _cat_cols(grads, ctx.widths, grads[0].shape[0], full, 0)
+        return full, None
+
+
+def ssm_head(out, head):
+    """aggregation_type == "ssm" head of one block: frames (mean over frequency, LayerNorm) -> projection to x | z -> causal convolution + SiLU
+    over x -> selective scan gated by z -> mean over the frames.  `head` = networks.classifiers.SsmHead (parameter holder); `out` (N, C, H, W)
+    block output (H == 1 for the 1-d model).  Returns (N, head.inner)."""
+    _need_cuda(out, "ssm_head")
+    n, _, _, w = out.shape
+    e, r, s = head.inner, head.rank, head.states
+    xl = FrameNormFn.apply(out, head.norm.eps, head.norm.weight, head.norm.bias)
+    x, z = SplitColsFn.apply(linear(xl.view(n * w, -1), head.in_proj.weight, head.in_proj.bias), (e, e))
+    x = causal_conv(x.view(n, w, e), head.conv_weight, head.conv_bias)
+    dt, b, c = SplitColsFn.apply(linear(x.view(n * w, e), head.x_proj.weight, None), (r, s, s))
+    dt = linear(dt, head.dt_proj.weight, None)
+    y = selective_scan(x, dt.view(n, w, e), head.a_log, b.view(n, w, s), c.view(n, w, s), d=head.d, z=z.view(n, w, e), dt_bias=head.dt_proj.bias)
+    return FrameMeanFn.apply(y)
 
 
 # ------------------------------------------------------------------------------ conv block

@@ -22,7 +22,7 @@ import torch.nn as nn
 
 from .. import functional as F
 from .. import parallel
-from ..ops.training import OPTIMIZERS, make_scheduler, make_step
+from ..ops.training import make_optimizer, make_scheduler, make_step
 from ..ops.utils import is_mel, is_stft, lwlrap, make_mel_filterbanks, parse_features
 from .losses import binary_cross_entropy, lsep_loss
 
@@ -75,6 +75,32 @@ class ResnetBlock2d(_ResidualHolder):
         super().__init__(depth, nn.Conv2d, nn.BatchNorm2d)
 
 
+class SsmHead(nn.Module):
+    """Parameter holder of the state-space aggregation head (aggregation_type "ssm", beside the reference's "max" and "rnn"); the
+    arithmetic lives in functional.ssm_head.  Time constants start log-uniform between 10 and 1000 frames, the state's rates at
+    1 .. states; both and the skip are kept out of the weight decay."""
+
+    def __init__(self, depth, inner=256, states=16, rank=16, taps=4):
+        super().__init__()
+        self.inner, self.states, self.rank = inner, states, rank
+        self.norm = nn.LayerNorm((depth,))
+        self.in_proj = nn.Linear(depth, 2 * inner)
+        bound = taps ** -0.5
+        self.conv_weight = nn.Parameter(torch.empty(inner, taps).uniform_(-bound, bound))
+        self.conv_bias = nn.Parameter(torch.zeros(inner))
+        self.x_proj = nn.Linear(inner, rank + 2 * states, bias=False)
+        self.dt_proj = nn.Linear(rank, inner)
+        rate = torch.exp(torch.empty(inner).uniform_(float(np.log(1e-3)), float(np.log(1e-1))))
+        with torch.no_grad():
+            self.dt_proj.bias.copy_(rate + torch.log(-torch.expm1(-rate)))          # softplus(bias) = rate
+        self.a_log = nn.Parameter(torch.log(torch.arange(1, states + 1, dtype=torch.float32)).repeat(inner, 1))
+        self.d = nn.Parameter(torch.ones(inner))
+        self.a_log.no_decay = self.d.no_decay = True
+
+    def forward(self, x):
+        raise RuntimeError("the head runs inside functional.ssm_head")
+
+
 class _TaggingModel(nn.Module):
     dims = 2
 
@@ -86,8 +112,8 @@ class _TaggingModel(nn.Module):
         self.loss_name = loss
         net, data = self.config.network, self.config.data
         self.aggregation = getattr(net, "aggregation_type", "max")
-        if self.aggregation not in ("max", "rnn"):
-            raise ValueError("aggregation_type must be 'max' or 'rnn', got %r" % (self.aggregation,))
+        if self.aggregation not in ("max", "rnn", "ssm"):
+            raise ValueError("aggregation_type must be 'max', 'rnn' or 'ssm', got %r" % (self.aggregation,))
         if torch.device(device).type != "cuda":
             raise F._lib.FscError("the accelerated model needs device='cuda' (an MI355X under ROCm); "
                                   "there is no CPU fallback")
@@ -100,6 +126,8 @@ class _TaggingModel(nn.Module):
         res = ResnetBlock2d if self.dims == 2 else ResnetBlock
         self.conv_modules = nn.ModuleList()
         self.rnns = nn.ModuleList()
+        if self.aggregation == "ssm":
+            self.ssms = nn.ModuleList()
         total_depth = 0
         depth = None
         for k in range(net.num_conv_blocks):
@@ -108,6 +136,9 @@ class _TaggingModel(nn.Module):
             if k >= net.start_deep_supervision_on:
                 if self.aggregation == "max":
                     total_depth += depth
+                elif self.aggregation == "ssm":
+                    self.ssms.append(SsmHead(depth))
+                    total_depth += self.ssms[-1].inner
                 else:                              # (created BEFORE the block's conv modules, like the reference: :514-522)
                     rnn_size = 128
                     total_depth += rnn_size * 2
@@ -197,6 +228,8 @@ class _TaggingModel(nn.Module):
             h, feat = F.conv_block(h, mods, self.training, use_max, ph, self._bn_sync, next_bn=k + 1 < len(self.conv_modules))
             if k >= start and self.aggregation == "rnn":
                 feat = F.rnn_head(h, self.rnns[k - start])
+            if k >= start and self.aggregation == "ssm":
+                feat = F.ssm_head(h, self.ssms[k - start])
             if feat is not None:
                 feats.append(feat)
         feats = F.cat_features(feats)
@@ -387,8 +420,7 @@ class _TaggingModel(nn.Module):
         train = self.config.train
         if self._reducer is not None:              # (a second call on the same model: drop the previous reducer's hooks first)
             self.close()
-        self.optimizer = OPTIMIZERS[train.optimizer](
-            self.parameters(), train.learning_rate, weight_decay=train.weight_decay)
+        self.optimizer = make_optimizer(train.optimizer, self, train.learning_rate, train.weight_decay)
         self.scheduler = make_scheduler(train.scheduler, max_steps=max_steps)(self.optimizer)
         # FSC_FORCE_DP=1 exercises the data-parallel path in a 1-rank process group (device test)
         if parallel.world_size() > 1 or (parallel.initialized() and os.environ.get("FSC_FORCE_DP") == "1"):

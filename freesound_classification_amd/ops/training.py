@@ -8,6 +8,7 @@ import os
 import warnings
 from functools import partial
 
+import numpy as np
 import torch
 from torch.optim import Optimizer
 from torch.optim.lr_scheduler import StepLR
@@ -138,10 +139,151 @@ class FusedSGD(Optimizer):
         return loss
 
 
+_PARAM_DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+STATE_BLOCK = 256        # elements that share one scale of an 8-bit moment
+
+
+class FusedAdamW(Optimizer):
+    """AdamW (torch.optim.AdamW's rule: weight decay apart from the moments) over all tensors of a group in one launch per 52 tensors.
+
+    `state_bits=32`: state keys match torch (step, exp_avg, exp_avg_sq), moments in fp32.  `state_bits=8`: the moments are held as e4m3 values
+    with one fp32 scale per 256 elements -- exp_avg / exp_avg_scale, and the square root of the second moment, exp_avg_sq_root /
+    exp_avg_sq_root_scale --, 2.03 bytes a parameter instead of 8, rounded stochastically: the random bits are a function of (`seed`, the
+    tensor's place in the optimizer, the step, the element), so a run is reproducible.  Parameters and gradients are fp32, bf16 or fp16.
+    `grad_scale` multiplies gradients first (1 / world_size after a summing all-reduce)."""
+
+    def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, state_bits=32, seed=0):
+        if state_bits not in (32, 8):
+            raise ValueError("state_bits must be 32 or 8, got %r" % (state_bits,))
+        if not (lr >= 0.0 and eps >= 0.0 and weight_decay >= 0.0 and all(0.0 <= b < 1.0 for b in betas)):
+            raise ValueError("FusedAdamW: lr, eps and weight_decay must be >= 0 and the betas in [0, 1)")
+        super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay))
+        self.state_bits = state_bits
+        self.seed = int(seed)
+        self.grad_scale = 1.0
+        self.factors_dev = None      # set while a step is recorded into a HIP graph: four floats a group in device memory
+
+    def _keys(self):
+        return ("exp_avg", "exp_avg_sq") if self.state_bits == 32 else ("exp_avg", "exp_avg_sq_root", "exp_avg_scale", "exp_avg_sq_root_scale")
+
+    def _new_state(self, p):
+        st = {"step": 0}
+        blocks = -(-p.numel() // STATE_BLOCK)
+        for key in self._keys():
+            if key.endswith("_scale"):
+                st[key] = torch.zeros(blocks, device=p.device, dtype=torch.float32)
+            else:
+                st[key] = torch.zeros(p.shape, device=p.device, dtype=torch.float32 if self.state_bits == 32 else torch.float8_e4m3fn)
+        return st
+
+    @torch.no_grad()
+    def step(self, closure=None):
+        loss = None
+        if closure is not None:
+            with torch.enable_grad():
+                loss = closure()
+        _forget_packed_weights()
+        ordinal = 0
+        for gi, group in enumerate(self.param_groups):
+            batches = {}                         # (dtype, step) -> [(parameter, gradient, state, place)]: one launch sequence each
+            for p in group["params"]:
+                ordinal += 1
+                g = p.grad
+                if g is None or p.numel() == 0:
+                    continue
+                if p.dtype not in _PARAM_DTYPES:
+                    raise _lib.FscError("FusedAdamW: parameters are fp32, bf16 or fp16, got %s" % p.dtype)
+                if g.is_sparse or not p.is_cuda or not g.is_contiguous():
+                    g = _checked_grad(p)
+                if not p.is_contiguous():
+                    raise _lib.FscError("FusedAdamW: parameters must be contiguous")
+                st = self.state[p]
+                if not st:
+                    st.update(self._new_state(p))
+                st["step"] = step = int(st["step"]) + 1
+                batches.setdefault((p.dtype, step), []).append((p, g, st, ordinal - 1))
+            for (dtype, step), entries in batches.items():
+                self._launch(gi, group, dtype, step, entries)
+        return loss
+
+    def _launch(self, gi, group, dtype, step, entries):
+        device = entries[0][0].device
+        if any(p.device != device for p, _, _, _ in entries) or device.index != _lib._get_device():
+            raise _lib.FscError("FusedAdamW: the parameters of a group must be on the current device")
+        n = len(entries)
+        table = np.zeros((n, 8), dtype=np.int64)
+        table[:, 0] = [e[0].data_ptr() for e in entries]
+        table[:, 1] = [e[1].data_ptr() for e in entries]
+        for column, key in enumerate(self._keys()):
+            table[:, 2 + column] = [e[2][key].data_ptr() for e in entries]
+        table[:, 6] = [e[0].numel() for e in entries]
+        table[:, 7] = [(self.seed + e[3]) & 0xFFFFFFFF for e in entries]
+        b1, b2 = group["betas"]
+        factors, dev = None, None
+        if self.factors_dev is not None:
+            dev = self.factors_dev.data_ptr() + 16 * gi
+        else:
+            factors = (C.c_float * 4)()
+            _lib.load().fsc_adamw_step_factors(float(group["lr"]), b1, b2, float(group["weight_decay"]), step, factors)
+        from .. import functional as F
+        count = int(table[:, 6].sum())
+        held = 8 if self.state_bits == 32 else 2
+        with F._stage("optimizer", count * (3 * entries[0][0].element_size() + 2 * held)):
+            call("fsc_adamw_step", table.ctypes.data, n, _PARAM_DTYPES[dtype], self.state_bits, factors, dev, b1, b2,
+                 float(group["eps"]), float(self.grad_scale), stream_ptr())
+
+    def state_dict(self):
+        out = super().state_dict()
+        out["state_bits"], out["seed"] = self.state_bits, self.seed
+        return out
+
+    def load_state_dict(self, state_dict):
+        """Like torch's, but the moments keep the types they are held in (torch casts floating state to the parameter's type)."""
+        if state_dict.get("state_bits", 32) != self.state_bits:
+            raise ValueError("FusedAdamW: the checkpoint holds its moments in %d bits, the optimizer in %d"
+                             % (state_dict.get("state_bits", 32), self.state_bits))
+        super().load_state_dict({k: v for k, v in state_dict.items() if k in ("state", "param_groups")})
+        self.seed = int(state_dict.get("seed", self.seed))
+        params = [p for group in self.param_groups for p in group["params"]]
+        places = [i for group in state_dict["param_groups"] for i in group["params"]]
+        for p, place in zip(params, places):
+            saved = state_dict["state"].get(place)
+            if not saved:
+                continue
+            fresh = self._new_state(p)
+            for key in self._keys():
+                if tuple(saved[key].shape) != tuple(fresh[key].shape):
+                    raise ValueError("FusedAdamW: %s of parameter %d has shape %s, expected %s"
+                                     % (key, place, tuple(saved[key].shape), tuple(fresh[key].shape)))
+                fresh[key].copy_(saved[key])
+            self.state[p] = dict(fresh, step=int(saved["step"]))
+
+
 OPTIMIZERS = {
     "adam": partial(FusedAdam, amsgrad=True),
     "momentum": partial(FusedSGD, momentum=0.9, nesterov=True),
 }
+# Optimizers that the reference does not have.  Their weight decay is for the weights alone: make_optimizer gives them two groups.
+DECOUPLED_OPTIMIZERS = {
+    "adamw": FusedAdamW,
+    "adamw8": partial(FusedAdamW, state_bits=8),
+}
+
+
+def decay_groups(named_parameters, weight_decay):
+    """Parameter groups for a decoupled optimizer: matrices and convolution filters decay; biases, norms, PReLU slopes and the time
+    constants of a state-space head (marked `no_decay`) do not."""
+    decay, rest = [], []
+    for _, p in named_parameters:
+        (decay if p.dim() > 1 and not getattr(p, "no_decay", False) else rest).append(p)
+    return [g for g in (dict(params=decay, weight_decay=weight_decay), dict(params=rest, weight_decay=0.0)) if g["params"]]
+
+
+def make_optimizer(name, module, lr, weight_decay):
+    """The optimizer `name` over a module's parameters: OPTIMIZERS as in the reference, DECOUPLED_OPTIMIZERS with their two groups."""
+    if name in DECOUPLED_OPTIMIZERS:
+        return DECOUPLED_OPTIMIZERS[name](decay_groups(module.named_parameters(), weight_decay), lr, weight_decay=weight_decay)
+    return OPTIMIZERS[name](module.parameters(), lr, weight_decay=weight_decay)
 
 
 class OneCycleScheduler:
@@ -201,7 +343,7 @@ class CapturedTrainingStep:
     What makes it legal: every entry point of libfsc_hip.so is capture-safe (include/fsc_hip.h: no allocation, no
     synchronisation, no host read-back); the step-dependent scalars of Adam travel through two device floats
     (fsc_adam_amsgrad_step_dev) refreshed in front of each replay; BatchNorm counters are bumped by a kernel.  What it needs:
-    fixed batch shape, Adam, accumulation_steps == 1, no dropout (its counter-based stream takes the offset by value), single
+    fixed batch shape, Adam or AdamW, accumulation_steps == 1, no dropout (its counter-based stream takes the offset by value), single
     GPU (no reducer), at least one eager step before (lazy state exists).  `model.training_step` semantics otherwise: returns
     (class_logits, per-sample loss, loss) -- static tensors, valid until the next call.
 
@@ -220,26 +362,30 @@ class CapturedTrainingStep:
 
     def __init__(self, model, signal, labels):
         opt = model.optimizer
-        if not isinstance(opt, FusedAdam):
-            raise _lib.FscError("CapturedTrainingStep needs the fused Adam optimizer")
+        if not isinstance(opt, (FusedAdam, FusedAdamW)):
+            raise _lib.FscError("CapturedTrainingStep needs the fused Adam or AdamW optimizer")
         if model._reducer is not None or model.config.train.accumulation_steps != 1:
             raise _lib.FscError("CapturedTrainingStep: single GPU, accumulation_steps == 1")
         if float(model.config.network.output_dropout) > 0.0:
             raise _lib.FscError("CapturedTrainingStep: dropout draws from a host-side counter; capture needs output_dropout == 0")
-        if len(opt.param_groups) != 1 or not all(opt.state[p] for p in opt.param_groups[0]["params"] if p.requires_grad):
+        decoupled = isinstance(opt, FusedAdamW)
+        trained = [p for group in opt.param_groups for p in group["params"] if p.requires_grad]
+        if (len(opt.param_groups) != 1 and not decoupled) or not all(opt.state[p] for p in trained):
             raise _lib.FscError("CapturedTrainingStep: run one eager training step first (optimizer state must exist)")
+        if decoupled and len({int(opt.state[p]["step"]) for p in trained}) != 1:
+            raise _lib.FscError("CapturedTrainingStep: the parameters have taken different numbers of steps")
         stream = torch.cuda.current_stream(signal.device)
         if stream == torch.cuda.default_stream(signal.device):
             raise _lib.FscError("CapturedTrainingStep: run the training loop -- eager steps, this constructor, the replays -- inside "
                                 "ONE `with torch.cuda.stream(s):` (not on the default stream; see the class docstring)")
         self.stream = stream
         self.model, self.opt = model, opt
-        self.group = opt.param_groups[0]
         self.step_count = int(next(iter(opt.state.values()))["step"])
         self.signal = signal.clone()
         self.labels = labels.clone()
-        self.factors = torch.zeros(2, device=signal.device, dtype=torch.float32)
-        self._buf = (C.c_float * 2)()
+        per_group = 4 if decoupled else 2
+        self.factors = torch.zeros(per_group * len(opt.param_groups), device=signal.device, dtype=torch.float32)
+        self._buf = (C.c_float * per_group)()
         self.graph = torch.cuda.CUDAGraph()
         opt.zero_grad()
         from .. import functional
@@ -280,11 +426,17 @@ class CapturedTrainingStep:
         functional.forget_packed_weights()
         for st in self.opt.state.values():                # (a checkpoint saved mid-run resumes with the right bias correction)
             st["step"] = self.step_count
-        b1, b2 = self.group["betas"]
-        _lib.load().fsc_adam_step_factors(float(self.group["lr"]), b1, b2, self.step_count, self._buf)
-        # (by-value kernel arguments: no host buffer that a later call could overwrite before an earlier copy has run)
-        call("fsc_fill", self.factors.data_ptr(), float(self._buf[0]), 1, stream_ptr())
-        call("fsc_fill", self.factors.data_ptr() + 4, float(self._buf[1]), 1, stream_ptr())
+        to = self.factors.data_ptr()
+        for group in self.opt.param_groups:
+            b1, b2 = group["betas"]
+            if isinstance(self.opt, FusedAdamW):
+                _lib.load().fsc_adamw_step_factors(float(group["lr"]), b1, b2, float(group["weight_decay"]), self.step_count, self._buf)
+            else:
+                _lib.load().fsc_adam_step_factors(float(group["lr"]), b1, b2, self.step_count, self._buf)
+            # (by-value kernel arguments: no host buffer that a later call could overwrite before an earlier copy has run)
+            for value in self._buf:
+                call("fsc_fill", to, float(value), 1, stream_ptr())
+                to += 4
         self.graph.replay()
         return self.outputs
 

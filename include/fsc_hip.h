@@ -543,6 +543,74 @@ int fsc_gru_step_bwd(const float* dh, const float* r_save, const float* z_save, 
                      long dgx_stride, float* dgh, float* dh_prev, int batch, int hidden,
                      fsc_stream_t stream);
 
+/* ------------------------------------------------------------------ sequence operators of the state-space head
+ * aggregation_type == "ssm" (beside "max" and "rnn"): the frames of a block through a short causal convolution and a selective
+ * scan.  Sequences are (batch, length, channels) with the channels contiguous; x / u / dt / z / b / c / dy are read through
+ * element strides of their batch and time axes (halves of one projection need no copy), everything written is contiguous.
+ * Activations are fp32, bf16 or fp16 (`dtype`), parameters, states and all sums fp32, one rounding at each output.
+ * lengths (batch, int32; NULL = full): frames t >= lengths[n] do not exist -- they are not read, their outputs and gradients are 0
+ * and states pass by them; values outside 0 .. length are clamped.  Zero batch, length or channels are legal. */
+#define FSC_DTYPE_F32 0
+#define FSC_DTYPE_BF16 1
+#define FSC_DTYPE_F16 2
+
+/* Causal convolution along time, one filter of 1 <= taps <= 8 a channel:
+ *   pre[n,t,c] = bias[c] + sum_k weight[c,k] xin[n, t + k, c],   xin = [initial (taps - 1 frames) | x],   y = silu(pre) or pre
+ *   final = the last taps - 1 frames of xin in front of lengths[n].
+ * Backward: dx, dinitial, dweight, dbias from dy and dfinal (either may be NULL: 0); no atomics, so equal inputs give equal bits. */
+typedef struct {
+    int batch, length, channels, taps, dtype, silu;
+    const void* x;
+    long x_batch, x_time;
+    const float *weight, *bias;  /* (channels, taps); (channels) or NULL */
+    const int* lengths;          /* or NULL */
+    const void* initial;         /* (batch, taps - 1, channels) or NULL: zeros */
+    void *y, *final;             /* forward: (batch, length, channels); (batch, taps - 1, channels) or NULL */
+    const void* dy;              /* backward */
+    long dy_batch, dy_time;
+    const void* dfinal;
+    void *dx, *dinitial;         /* dinitial may be NULL */
+    float *dweight, *dbias;      /* dbias may be NULL */
+    void* workspace;             /* fsc_causal_conv_bwd_workspace_bytes */
+} fsc_causal_conv_args;
+int fsc_causal_conv_fwd(const fsc_causal_conv_args* args_host, fsc_stream_t stream);
+size_t fsc_causal_conv_bwd_workspace_bytes(const fsc_causal_conv_args* args_host);
+int fsc_causal_conv_bwd(const fsc_causal_conv_args* args_host, fsc_stream_t stream);
+/* One frame: x, y (batch, channels), window (batch, taps - 1, channels) = `initial`, shifted by one frame in place (`length` is ignored). */
+int fsc_causal_conv_step(const fsc_causal_conv_args* args_host, fsc_stream_t stream);
+
+/* Selective scan, 1 <= states <= 64 a channel, channels in `groups` equal groups that share b and c:
+ *   delta = softplus(dt + dt_bias) (softplus == 0: dt + dt_bias),  A = -exp(a_log)
+ *   h[n,t,c,s] = exp(delta A[c,s]) h[n,t-1,c,s] + delta u[n,t,c] b[n,t,g,s],   h[n,-1] = initial or 0
+ *   y[n,t,c] = (sum_s c[n,t,g,s] h[n,t,c,s] + d[c] u[n,t,c]) silu(z[n,t,c])      (d, z NULL: without)
+ *   final = h behind the last frame.
+ * The forward with `checkpoints` (fsc_selective_scan_checkpoint_bytes) keeps what the backward needs; backward: every gradient
+ * from dy and dfinal (either may be NULL: 0), without atomics. */
+typedef struct {
+    int batch, length, channels, states, groups, dtype, softplus;
+    const void *u, *dt, *z, *b, *c;
+    long u_batch, u_time, dt_batch, dt_time, z_batch, z_time, b_batch, b_time, b_group, c_batch, c_time, c_group;
+    const float *a_log, *d, *dt_bias;  /* (channels, states); (channels) or NULL; (channels) or NULL */
+    const int* lengths;                /* or NULL */
+    const float* initial;              /* (batch, channels, states) or NULL */
+    void* y;                           /* forward */
+    float* final;                      /* (batch, channels, states) or NULL */
+    float* checkpoints;                /* forward writes (NULL: inference), backward reads */
+    void* workspace;                   /* fsc_selective_scan_workspace_bytes(args, backward) */
+    const void* dy;                    /* backward */
+    long dy_batch, dy_time;
+    const float* dfinal;
+    void *du, *ddt, *dz, *db, *dc;     /* dz may be NULL only without z; db / dc (batch, length, groups, states) */
+    float *da_log, *dd, *ddt_bias, *dinitial;  /* dd, ddt_bias, dinitial may be NULL */
+} fsc_selective_scan_args;
+size_t fsc_selective_scan_checkpoint_bytes(const fsc_selective_scan_args* args_host);
+size_t fsc_selective_scan_workspace_bytes(const fsc_selective_scan_args* args_host, int backward);
+int fsc_selective_scan_fwd(const fsc_selective_scan_args* args_host, fsc_stream_t stream);
+int fsc_selective_scan_bwd(const fsc_selective_scan_args* args_host, fsc_stream_t stream);
+/* One frame: u, dt, z, y (batch, channels), b, c (batch, groups, states); `final` (batch, channels, states) is the state, updated in
+ * place (`length`, `lengths`, `initial` and the time strides are ignored). */
+int fsc_selective_scan_step(const fsc_selective_scan_args* args_host, fsc_stream_t stream);
+
 /* ------------------------------------------------------------------ optimizers (K16)
  * ops/training.py:9-12: Adam(amsgrad=True) and SGD(momentum=0.9, nesterov=True), both with
  * L2 weight decay folded into the gradient (torch semantics). */
@@ -574,6 +642,27 @@ int fsc_adam_amsgrad_step_dev(const fsc_opt_tensor* tensors_host, int n_tensors,
 int fsc_sgd_nesterov_step(const fsc_opt_tensor* tensors_host, int n_tensors, float lr,
                           float momentum, float weight_decay, int first_step,
                           float grad_scale, fsc_stream_t stream);
+
+/* AdamW (weight decay apart from the moments) over many tensors, parameters and gradients in one of FSC_DTYPE_*, arithmetic fp32:
+ *   p <- p decay - step_size m / (sqrt(v) inv_root + eps),   m <- m beta1 + g (1 - beta1),   v <- v beta2 + g g (1 - beta2),
+ *   decay = 1 - lr weight_decay, step_size = lr / (1 - beta1^step), inv_root = 1 / sqrt(1 - beta2^step), g = grad * grad_scale.
+ * state_bits 32: state0 = m, state1 = v (fp32).  state_bits 8: state0 / state1 = e4m3 values of m / sqrt(v), scale0 / scale1 one fp32
+ * scale for each 256 elements; each value is rounded down or up with the probability of its remainder, from 16 bits of a counter-based
+ * hash of (salt, step modulo 2^24, element), and a second moment above 0 is never held as 0.  A value that is not finite is held as NaN
+ * and leaves its block's scale alone. */
+typedef struct {
+    void* param;
+    const void* grad;
+    void *state0, *state1;
+    float *scale0, *scale1; /* state_bits 8 */
+    long count;             /* 0 is legal: skipped */
+    unsigned long salt;     /* its low 32 bits: what tells this tensor's random bits from another's */
+} fsc_adamw_tensor;
+/* factors4 = {decay, step_size, inv_root, step modulo 2^24}: HOST floats, or NULL and factors4_dev in DEVICE memory (a step recorded into a
+ * HIP graph; the caller refreshes them in front of each replay). */
+void fsc_adamw_step_factors(double lr, double beta1, double beta2, double weight_decay, long step, float* out4_host);
+int fsc_adamw_step(const fsc_adamw_tensor* tensors_host, int n_tensors, int dtype, int state_bits, const float* factors4,
+                   const float* factors4_dev, double beta1, double beta2, float eps, float grad_scale, fsc_stream_t stream);
 
 /* ------------------------------------------------------------------ misc device helpers */
 /* out[c][8] (pre-zeroed) += per channel, over all images of x (N, C, H, W): sums of the first row, last row, first column,

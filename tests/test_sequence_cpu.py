@@ -1,0 +1,163 @@
+"""Sequence operators and AdamW without a device: argument checks of the Python layer and of the C ABI, plan arithmetic, the 8-bit format."""
+import ctypes as C
+
+import numpy as np
+import pytest
+import torch
+
+import freesound_classification_amd as pkg
+from freesound_classification_amd import _lib
+from freesound_classification_amd import functional as F
+from freesound_classification_amd.ops import training
+from oracle import sequence as oseq
+
+
+def _conv(**kw):
+    return _lib.CausalConvArgs(**dict(dict(batch=2, length=20, channels=8, taps=4), **kw))
+
+
+def _scan(**kw):
+    return _lib.ScanArgs(**dict(dict(batch=2, length=40, channels=8, states=16, groups=1, a_log=64), **kw))
+
+
+def _refused(name, *args, match):
+    lib = pkg.load_library()
+    assert getattr(lib, name)(*args) == 22
+    assert match in lib.fsc_last_error_string().decode()
+
+
+@pytest.mark.parametrize("name", ["fsc_causal_conv_fwd", "fsc_causal_conv_bwd", "fsc_causal_conv_step"])
+def test_conv_entry_points_refuse_bad_arguments(name):
+    _refused(name, None, None, match="null arguments")
+    for kw, text in ((dict(taps=0), "taps"), (dict(taps=9), "taps"), (dict(dtype=3), "dtype"), (dict(batch=-1), "negative"),
+                     (dict(), "null weight"), (dict(channels=(1 << 23) + 1, weight=64), "channels"),
+                     (dict(batch=2 ** 30, length=2 ** 30, weight=64), "too large"), (dict(weight=64), "null")):
+        _refused(name, C.byref(_conv(**kw)), None, match=text)
+
+
+@pytest.mark.parametrize("name", ["fsc_selective_scan_fwd", "fsc_selective_scan_bwd", "fsc_selective_scan_step"])
+def test_scan_entry_points_refuse_bad_arguments(name):
+    _refused(name, None, None, match="null arguments")
+    for kw, text in ((dict(states=0), "states"), (dict(states=65), "states"), (dict(groups=3), "groups"), (dict(groups=0), "groups"),
+                     (dict(dtype=-1), "dtype"), (dict(length=-1), "negative"), (dict(a_log=None), "a_log"),
+                     (dict(batch=2 ** 30), "too large"), (dict(), "null")):
+        _refused(name, C.byref(_scan(**kw)), None, match=text)
+
+
+def test_empty_calls_launch_nothing():
+    lib = pkg.load_library()
+    for kw in (dict(batch=0), dict(channels=0), dict(length=0)):
+        assert lib.fsc_causal_conv_fwd(C.byref(_conv(weight=64, **kw)), None) == 0
+        assert lib.fsc_selective_scan_fwd(C.byref(_scan(**kw)), None) == 0
+    assert lib.fsc_causal_conv_step(C.byref(_conv(weight=64, batch=0)), None) == 0
+    assert lib.fsc_selective_scan_step(C.byref(_scan(batch=0)), None) == 0
+
+
+def test_scan_plans():
+    """Kept states: one a tile of 16 frames, whole blocks of 64 channels (32 / 16 of them with more than 16 / 32 states).  Segments only
+    where sequences and channels leave the card empty; their ends cost workspace."""
+    lib = pkg.load_library()
+    kept = lambda **kw: lib.fsc_selective_scan_checkpoint_bytes(C.byref(_scan(**kw)))  # noqa: E731
+    ws = lambda back, **kw: lib.fsc_selective_scan_workspace_bytes(C.byref(_scan(**kw)), back)  # noqa: E731
+    assert kept(batch=3, length=33, channels=65, states=16) == 4 * 3 * 3 * 128 * 16
+    assert kept(batch=3, length=33, channels=65, states=5) == 4 * 3 * 3 * 128 * 8
+    assert kept(batch=1, length=1, channels=1, states=64) == 4 * 16 * 64
+    assert kept(batch=1, length=16, channels=66, states=20, groups=2) == 4 * 128 * 32
+    assert kept(length=0) == 0
+    assert ws(0, batch=4096, length=512) == 0 and ws(0, batch=1, length=512) > 0
+    assert ws(1, batch=4096, length=512) > 0
+    assert ws(0, states=65) == 0
+
+
+def test_adamw_entry_point_refuses_bad_arguments():
+    entry = (C.c_int64 * 8)(64, 64, 64, 64, 0, 0, 10, 0)
+    factors = (C.c_float * 4)()
+    call = lambda table, n, dtype, bits, f, dev: ("fsc_adamw_step", table, n, dtype, bits, f, dev, 0.9, 0.999, 1e-8, 1.0, None)  # noqa: E731
+    _refused(*call(None, 1, 0, 32, factors, None), match="bad arguments")
+    _refused(*call(entry, 0, 0, 32, factors, None), match="bad arguments")
+    _refused(*call(entry, 1, 0, 32, None, None), match="bad arguments")
+    _refused(*call(entry, 1, 0, 32, factors, 64), match="bad arguments")
+    _refused(*call(entry, 1, 5, 32, factors, None), match="dtype")
+    _refused(*call(entry, 1, 0, 16, factors, None), match="state_bits")
+    _refused(*call(entry, 1, 0, 8, factors, None), match="scales")
+    entry[6] = -1
+    _refused(*call(entry, 1, 0, 32, factors, None), match="elements")
+    entry[6], entry[3] = 10, 0
+    _refused(*call(entry, 1, 0, 32, factors, None), match="null pointers")
+    entry[6] = 0                                                             # an empty tensor is skipped
+    assert pkg.load_library().fsc_adamw_step(entry, 1, 0, 32, factors, None, 0.9, 0.999, 1e-8, 1.0, None) == 0
+
+
+def test_adamw_step_factors():
+    out = (C.c_float * 4)()
+    pkg.load_library().fsc_adamw_step_factors(3e-3, 0.9, 0.999, 0.01, 2 ** 24 + 7, out)
+    f = np.float32
+    assert list(out) == [f(1 - 3e-3 * 0.01), f(3e-3), f(1.0), f(7)]
+    pkg.load_library().fsc_adamw_step_factors(3e-3, 0.9, 0.999, 0.0, 3, out)
+    assert list(out) == [f(1), f(3e-3 / (1 - 0.9 ** 3)), f(1 / np.sqrt(1 - 0.999 ** 3)), f(3)]
+
+
+def test_operators_need_a_device():
+    x = torch.zeros(2, 5, 8)
+    w = torch.zeros(8, 4)
+    a = torch.zeros(8, 16)
+    rows = torch.zeros(2, 5, 16)
+    for fn in (lambda: F.causal_conv(x, w), lambda: F.causal_conv_step(x[:, 0], torch.zeros(2, 3, 8), w), lambda: F.selective_scan(x, x, a, rows, rows),
+               lambda: F.selective_scan_step(x[:, 0], x[:, 0], a, rows[:, 0], rows[:, 0], torch.zeros(2, 8, 16))):
+        with pytest.raises(_lib.FscError, match="device tensor"):
+            fn()
+    for fn in (lambda: F.causal_conv(x[0], w), lambda: F.causal_conv(x, w, activation="gelu"), lambda: F.selective_scan(x[0], x[0], a, rows, rows)):
+        with pytest.raises(_lib.FscError):
+            fn()
+
+
+def test_optimizer_registry_and_groups():
+    assert set(training.DECOUPLED_OPTIMIZERS) == {"adamw", "adamw8"}
+    m = torch.nn.Sequential(torch.nn.Conv2d(2, 3, 3), torch.nn.BatchNorm2d(3), torch.nn.Linear(3, 4))
+    m[2].weight.no_decay = True
+    opt = training.make_optimizer("adamw8", m, 1e-3, 0.1)
+    assert opt.state_bits == 8 and [g["weight_decay"] for g in opt.param_groups] == [0.1, 0.0]
+    assert opt.param_groups[0]["params"] == [m[0].weight] and len(opt.param_groups[1]["params"]) == 5
+    assert isinstance(training.make_optimizer("adam", m, 1e-3, 0.1), training.FusedAdam)
+    assert isinstance(training.make_optimizer("momentum", m, 1e-3, 0.1), training.FusedSGD)
+    with pytest.raises(KeyError):
+        training.make_optimizer("lion", m, 1e-3, 0.1)
+    for kw in (dict(state_bits=4), dict(lr=-1.0), dict(betas=(1.0, 0.9)), dict(eps=-1e-8), dict(weight_decay=-1.0)):
+        with pytest.raises(ValueError):
+            training.FusedAdamW(m.parameters(), **kw)
+    m[0].weight.grad = torch.zeros_like(m[0].weight)
+    with pytest.raises(_lib.FscError, match="device parameters"):
+        opt.step()
+
+
+def test_held_values():
+    """The 8-bit format's patterns are torch's e4m3; a value on the grid is held exactly whatever the random bits, one between two grid
+    points goes to the upper with the probability of its remainder: over all 2^16 random numbers, exactly that share of them."""
+    codes = np.arange(256, dtype=np.uint8)
+    want = torch.from_numpy(codes).view(torch.float8_e4m3fn).float().numpy()
+    assert np.array_equal(oseq.e4m3_value(codes), want, equal_nan=True)
+    grid = oseq.e4m3_value(np.arange(1, 0x7F, dtype=np.uint8))
+    for bits in (0, 1, 40000, 65535):
+        x = np.concatenate([grid, -grid, np.float32([0, 448])])
+        code, scale = oseq.held8(x, np.full(x.size, bits, dtype=np.uint32), False)
+        assert scale[0] == 1 and np.array_equal(oseq.e4m3_value(code), x)
+    every = np.arange(65536, dtype=np.uint32)
+    for lo, hi, share in ((16, 18, 0.25), (2.0 ** -9, 2.0 ** -8, 0.75), (15, 16, 0.5), (0, 2.0 ** -9, 0.125)):
+        x = np.full(65536, lo + share * (hi - lo), dtype=np.float32)
+        x[::256] = 448
+        code, _ = oseq.held8(x, every, False)
+        value = oseq.e4m3_value(code)
+        inner = np.arange(65536) % 256 != 0
+        assert set(np.unique(value[inner])) == {np.float32(lo), np.float32(hi)}
+        assert abs(np.mean(value[inner] == hi) - share) < 1 / 256 + 1e-6      # (the 256 places of the maxima are not looked at)
+
+
+def test_random_bits_are_spread():
+    """Bits of neighbouring elements, steps and tensors: every bit set in half of the numbers within five standard deviations."""
+    for salt, step in ((0, 1), (0, 2), (1, 1), (123456789, 16777215)):
+        bits = oseq.random_bits(salt, step, 1 << 16)
+        for i in range(32):
+            assert abs(float(np.mean((bits >> np.uint32(i)) & np.uint32(1))) - 0.5) < 5 * 0.5 / 256
+    a, b, c = (oseq.random_bits(*v, 1 << 16) for v in ((0, 1), (0, 2), (1, 1)))
+    for x, y in ((a, b), (a, c), (a[1:], a[:-1])):
+        assert abs(float(np.mean(np.bitwise_xor(x, y) & np.uint32(1))) - 0.5) < 5 * 0.5 / 256

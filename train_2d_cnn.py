@@ -57,7 +57,8 @@ def build_parser(default_label="2d_cnn"):
                    help="the accelerated path runs on an MI355X (\"cuda\" under ROCm); \"cpu\" raises: there is no CPU fallback")
     p.add_argument("--gpus", type=int, default=1,
                    help="data-parallel ranks to start on this node (one process per GPU, RCCL gradient all-reduce); not a reference flag")
-    p.add_argument("--aggregation_type", type=str, default="max", choices=("max", "rnn"), help="how to aggregate outputs")
+    p.add_argument("--aggregation_type", type=str, default="max", choices=("max", "rnn", "ssm"),
+                   help="how to aggregate outputs (\"ssm\", a state-space head, is not a reference choice)")
     p.add_argument("--num_conv_blocks", type=int, default=5, help="number of conv blocks")
     p.add_argument("--start_deep_supervision_on", type=int, default=2,
                    help="from which layer to start aggregating features for classification")
@@ -69,7 +70,8 @@ def build_parser(default_label="2d_cnn"):
     p.add_argument("--p_aug", type=float, default=0.0, help="probability of audio augmentation (sox; not on the accelerated path)")
     p.add_argument("--switch_off_augmentations_on", type=int, default=20, help="on which epoch to remove augmentations")
     p.add_argument("--features", type=str, default="mel_2048_1024_128", help="feature descriptor")
-    p.add_argument("--optimizer", type=str, default="adam", help="which optimizer to use", choices=("adam", "momentum"))
+    p.add_argument("--optimizer", type=str, default="adam", choices=("adam", "momentum", "adamw", "adamw8"),
+                   help="which optimizer to use (adamw: decoupled weight decay; adamw8: the same with its moments in 8 bits; not reference choices)")
     p.add_argument("--folds", type=int, default=[0], nargs="+", help="which folds to use")
     p.add_argument("--n_folds", type=int, default=4, help="number of folds")
     p.add_argument("--kfold_seed", type=int, default=42, help="kfold seed")
@@ -252,7 +254,7 @@ def main(model_cls=TwoDimensionalCNNClassificationModel, default_label="2d_cnn",
                 SoundDataset(
                     audio_files=files, labels=labels, is_noisy=[0] * len(train) + [1] * len(noisy_labels),
                     transform=Compose(clean_tf + [
-                        ShuffleAudio(chunk_length=0.5, p=0.5) if config.network.aggregation_type != "rnn" else Identity(),
+                        ShuffleAudio(chunk_length=0.5, p=0.5) if config.network.aggregation_type == "max" else Identity(),
                         MixUp(p=args.p_mixup), audio_transform, drop]),
                     clean_transform=Compose(list(clean_tf))),
                 shuffle=True, drop_last=True, batch_size=config.train.batch_size, collate_fn=collate, **loader_kwargs)
