@@ -23,11 +23,15 @@ struct ScanPlan {
     int channels_block;                  // CB = 256 / L
     int group_channels, group_blocks;    // channels of a group, blocks of CB channels it takes
     int blocks;                          // groups * group_blocks
-    int tiles, segments, segment_tiles;
+    int tiles, segments;                 // of 16 frames, of the longest sequence; segments of time (each sequence's own length in equal parts)
     int wide;                            // E neighbouring channels can be read and written at once
     __host__ __device__ int padded_states() const { return lanes * per_lane; }
     __host__ __device__ long padded_channels() const { return (long)blocks * channels_block; }
 };
+
+// LDS rows and channels of a block.  An elementwise thread has E neighbouring channels (one wide load); their rows lie 16 apart, so that the 16
+// threads of a frame write neighbouring rows, which start in different banks: row r is channel (r % 16) E + r / 16.
+__host__ __device__ inline int channel_of(int row, int e) { return (row & 15) * e + (row >> 4); }
 
 inline ScanPlan scan_plan(const fsc_selective_scan_args& a) {
     ScanPlan p{};
@@ -38,15 +42,14 @@ inline ScanPlan scan_plan(const fsc_selective_scan_args& a) {
     p.group_blocks = ceil_div(p.group_channels, p.channels_block);
     p.blocks = a.groups * p.group_blocks;
     p.tiles = ceil_div(a.length, kTile);
+    // 1024 workgroups are four waves a SIMD.  Segments double the exponentials, so half of that is enough not to cut.
     const long have = (long)a.batch * p.blocks, wanted = 1024;
     p.segments = 1;
-    if (have * 2 <= wanted && p.tiles >= 4) {
+    if (have * 2 < wanted && p.tiles >= 4) {
         long want = (wanted + have - 1) / have, most = p.tiles / 2;
         if (most > 32) most = 32;
         p.segments = (int)(want < most ? want : most);
     }
-    p.segment_tiles = p.tiles > 0 ? ceil_div(p.tiles, p.segments) : 1;
-    p.segments = p.tiles > 0 ? ceil_div(p.tiles, p.segment_tiles) : 1;
     const int e = kTile / p.lanes;
     const size_t unit = e * dtype_bytes(a.dtype);
     auto fits = [&](const void* ptr, long batch, long time) { return ptr == nullptr || (aligned(ptr, unit) && batch % e == 0 && time % e == 0); };
@@ -65,6 +68,10 @@ inline const char* scan_bad(const fsc_selective_scan_args* a) {
     if (a->channels > 0 && a->a_log == nullptr) return "null a_log";
     if ((long)a->batch * ((a->channels / a->groups / 16 + 1) * (long)a->groups) > 0x3FFFFFFL || a->length > 0x7FFFFFF0)
         return "batch * channels or length is too large";
+    // a tile's rows are addressed by 32-bit offsets from its first
+    const long strides[] = {a->u_time, a->dt_time, a->z_time, a->b_time, a->c_time, a->dy_time, a->channels};
+    for (const long s : strides)
+        if (s < 0 || s > (1L << 26)) return "negative time strides, or time strides or channels above 2^26";
     return nullptr;
 }
 
@@ -74,17 +81,39 @@ __device__ __forceinline__ int scan_frames(const fsc_selective_scan_args& a, int
     return l < 0 ? 0 : l > a.length ? a.length : l;
 }
 
+// The (k % 4)-th of four frames' sums, which is the one that a lane writes.  (By value: a choice between elements of an array puts it in memory.)
+__device__ __forceinline__ float pick4(float v0, float v1, float v2, float v3, int k) {
+    const float low = k & 1 ? v1 : v0, high = k & 1 ? v3 : v2;
+    return k & 2 ? high : low;
+}
+
 __device__ __forceinline__ int tiles_with(int frames) { return (frames + kTile - 1) / kTile; }
 
 __device__ __forceinline__ float sigmoid_fast(float v) {
     return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(v * -kLog2e));
 }
 
-// log(1 + e^v).  log(w) e / (w - 1) with w = 1 + e^v as rounded: what the rounding of w loses cancels, so small values keep their bits.
-__device__ __forceinline__ float softplus_fast(float v) {
-    const float e = __builtin_amdgcn_exp2f(v * kLog2e), w = 1.0f + e;
-    const float soft = w == 1.0f ? e : __builtin_amdgcn_logf(w) * kLn2 * (e * __builtin_amdgcn_rcpf(w - 1.0f));
-    return v > 20.0f ? v : soft;
+// Time steps are held in units of ln 2: exp(delta A) = 2^(delta2 A), and ln 2 is folded into B where it is staged.
+// delta2 = log2(1 + 2^v2) = max(v2, 0) + log2(1 + e) with e = 2^-|v2| <= 1.  What the rounding of w = 1 + e loses, c = e - (w - 1), comes back as
+// c log2(e): small values keep their bits.
+__device__ __forceinline__ float softplus2(float v2) {
+    const float e = __builtin_amdgcn_exp2f(-fabsf(v2)), w = 1.0f + e;
+    return fmaxf(v2, 0.f) + fmaf(e - (w - 1.0f), kLog2e, __builtin_amdgcn_logf(w));
+}
+__device__ __forceinline__ float sigmoid2(float v2) { return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-v2)); }
+
+// delta2 of E channels of a frame; 0 where the frame does not exist, so that the state passes it unchanged.  (The uniform choice stands outside the
+// loop: the E chains of transcendentals then run side by side.)
+template <int E, typename T>
+__device__ __forceinline__ void time_steps(const Pack<T, E>& dt, const float (&bias2)[E], bool soft, bool there, float (&raw)[E], float (&delta)[E]) {
+#pragma unroll
+    for (int i = 0; i < E; ++i) delta[i] = raw[i] = fmaf((float)dt.v[i], kLog2e, bias2[i]);
+    if (soft) {
+#pragma unroll
+        for (int i = 0; i < E; ++i) delta[i] = softplus2(raw[i]);
+    }
+#pragma unroll
+    for (int i = 0; i < E; ++i) delta[i] = there ? delta[i] : 0.f;
 }
 
 // Where a workgroup and its threads stand.
@@ -94,9 +123,12 @@ struct ScanPlace {
     int n, block, segment;       // sequence, channel block, segment of time
     int group, c0, have;         // channel group; first channel of the block, its channels that exist
     int te, ce, he;              // elementwise: frame in the tile, first channel in the block, how many of the E exist
-    int ch, sg, channel;         // scan: channel in the block, share of the states; channel index (clamped for lanes without one)
+    int ch, sg, channel;         // scan: LDS row, share of the states; channel (of the first row for lanes without one)
+    int first, work_end;         // the segment's tiles: the frames of the sequence in equal parts
+    int zero_first, zero_end;    // its share of the tiles behind the sequence's end, which only get zeros
+    bool whole;                  // every channel of the block exists and rows are read E channels at once
     bool real;                   // the scan lane has a channel
-    __device__ ScanPlace(const fsc_selective_scan_args& a, const ScanPlan& p) {
+    __device__ ScanPlace(const fsc_selective_scan_args& a, const ScanPlan& p, int& len) {
         // segments vary fastest but one: blocks of one sequence's segment, which read the same B and C, follow one another
         const int per = p.blocks * p.segments;
         n = blockIdx.x / per;
@@ -104,17 +136,26 @@ struct ScanPlace {
         segment = rest / p.blocks;
         block = rest % p.blocks;
         group = block / p.group_blocks;
+        len = scan_frames(a, n);
+        const int full = (len + kTile - 1) / kTile, part = (full + p.segments - 1) / p.segments, rest_part = (p.tiles - full + p.segments - 1) / p.segments;
+        first = segment * part < full ? segment * part : full;
+        work_end = first + part < full ? first + part : full;
+        zero_first = full + segment * rest_part < p.tiles ? full + segment * rest_part : p.tiles;
+        zero_end = zero_first + rest_part < p.tiles ? zero_first + rest_part : p.tiles;
         const int in_group = (block % p.group_blocks) * CB;
         c0 = group * p.group_channels + in_group;
         have = p.group_channels - in_group < CB ? p.group_channels - in_group : CB;
+        whole = p.wide && have == CB;
         te = threadIdx.x >> 4;
         ce = (threadIdx.x & 15) * E;
         he = have - ce < 0 ? 0 : have - ce < E ? have - ce : E;
         ch = threadIdx.x / L;
         sg = threadIdx.x % L;
-        real = ch < have;
-        channel = c0 + (real ? ch : 0);
+        real = channel_of(ch, E) < have;
+        channel = c0 + (real ? channel_of(ch, E) : 0);
     }
+    // LDS row of the elementwise thread's i-th channel
+    __device__ int lds_row(int i) const { return (threadIdx.x & 15) + 16 * i; }
     // element (row, state) of a B / C tile that this thread stages as its j-th
     __device__ int bc_row(int j) const { return (threadIdx.x + j * 256) / SP; }
     __device__ int bc_state(int j) const { return (threadIdx.x + j * 256) % SP; }
@@ -123,18 +164,90 @@ struct ScanPlace {
     __device__ long kept(const ScanPlan& p, int tile) const {
         return ((((long)n * p.blocks + block) * p.tiles + tile) * 256 + threadIdx.x) * NS;
     }
+    // ... among the partial sums of dB and dC [sequence][block][tile], each 16 x 2 x SP floats
+    __device__ long rows(const ScanPlan& p, int tile) const { return (((long)n * p.blocks + block) * p.tiles + tile) * (kTile * 2 * SP); }
     // ... and among the segments' ends [sequence][segment][block]
     __device__ long end(const ScanPlan& p, int seg) const { return ((((long)n * p.segments + seg) * p.blocks + block) * 256 + threadIdx.x) * NS; }
     __device__ long end_delta(const ScanPlan& p, int seg) const { return (((long)n * p.segments + seg) * p.blocks + block) * CB + ch; }
 };
 
-// -exp(a_log) log2(e) of the lane's states: exp(delta A) = 2^(delta A2).  0 for states that do not exist.
+// An activation as the elementwise threads read it: E channels of frame te of a tile, as they lie in memory (converted where they are used, so that
+// many loads are in flight).  The address is a uniform 64-bit one and a 32-bit offset of the thread; frames behind the last are read from
+// the last, channels that do not exist from the block's last (the caller leaves both out).
+template <typename T, int L, int NS>
+struct ScanFrames {
+    using Place = ScanPlace<L, NS>;
+    static constexpr int E = Place::E;
+    const char* base;
+    long time;
+    uint32_t off;
+    __device__ ScanFrames(const Place& w, const void* ptr, long batch, long time_) : time(time_ * (long)sizeof(T)) {
+        base = reinterpret_cast<const char*>(reinterpret_cast<const T*>(ptr) + w.n * batch + w.c0);
+        off = (uint32_t)w.te * (uint32_t)time + w.ce * (uint32_t)sizeof(T);
+    }
+    __device__ __forceinline__ void fetch(const Place& w, int tile, int len, Pack<T, E>& out) const {
+        const int last = len - 1 - tile * kTile;
+        const char* at = base + tile * kTile * time;
+        const uint32_t o = w.te <= last ? off : (uint32_t)last * (uint32_t)time + w.ce * (uint32_t)sizeof(T);
+        if (w.whole) {
+            out = load_pack<T, E>(reinterpret_cast<const T*>(at + o));
+        } else {
+#pragma unroll
+            for (int i = 0; i < E; ++i) {
+                const int c = w.ce + i < w.have ? w.ce + i : w.have - 1;
+                out.v[i] = *reinterpret_cast<const T*>(at + (o + (uint32_t)(c - w.ce) * (uint32_t)sizeof(T)));
+            }
+        }
+    }
+};
+
+// One tile of B or C as this thread stages it, in the same way; rows and states that do not exist are staged as 0, the others times `unit`.
+template <typename T, int L, int NS>
+struct ScanRows {
+    using Place = ScanPlace<L, NS>;
+    static constexpr int R = Place::ROWS;
+    const char* base;
+    long time;
+    uint32_t off[R], col[R];
+    T v[R];
+    __device__ ScanRows(const Place& w, const void* ptr, long batch, long time_, long group, int states) : time(time_ * (long)sizeof(T)) {
+        base = reinterpret_cast<const char*>(reinterpret_cast<const T*>(ptr) + w.n * batch + w.group * group);
+#pragma unroll
+        for (int j = 0; j < R; ++j) {
+            col[j] = (uint32_t)(w.bc_state(j) < states ? w.bc_state(j) : states - 1) * (uint32_t)sizeof(T);
+            off[j] = (uint32_t)row(w, j) * (uint32_t)time + col[j];
+        }
+    }
+    // (with fewer than 16 states some threads stage nothing; they read the tile's last row)
+    static __device__ int row(const Place& w, int j) { return w.bc_row(j) < kTile ? w.bc_row(j) : kTile - 1; }
+    __device__ __forceinline__ void fetch(const Place& w, int tile, int len) {
+        const int last = len - 1 - tile * kTile;
+        const char* at = base + tile * kTile * time;
+#pragma unroll
+        for (int j = 0; j < R; ++j)
+            v[j] = *reinterpret_cast<const T*>(at + (row(w, j) <= last ? off[j] : (uint32_t)last * (uint32_t)time + col[j]));
+    }
+    __device__ __forceinline__ void stage(const Place& w, float (*to)[Place::SP], int tile, int len, int states, float unit) const {
+#pragma unroll
+        for (int j = 0; j < R; ++j)
+            if (w.bc_mine(j)) to[w.bc_row(j)][w.bc_state(j)] = tile * kTile + w.bc_row(j) < len && w.bc_state(j) < states ? (float)v[j] * unit : 0.f;
+    }
+};
+
+// An output row (batch, length, channels) of frame te of a tile, first channel ce of the block.
+template <typename T, int L, int NS>
+__device__ __forceinline__ T* scan_out(const fsc_selective_scan_args& a, const ScanPlace<L, NS>& w, void* base, int tile) {
+    char* at = reinterpret_cast<char*>(reinterpret_cast<T*>(base) + ((long)w.n * a.length + (long)tile * kTile) * a.channels + w.c0);
+    return reinterpret_cast<T*>(at + ((uint32_t)w.te * (uint32_t)a.channels + w.ce) * (uint32_t)sizeof(T));
+}
+
+// A = -exp(a_log) of the lane's states, 0 for states that do not exist.
 template <int L, int NS>
-__device__ __forceinline__ void scan_rates(const fsc_selective_scan_args& a, const ScanPlace<L, NS>& w, float (&a2)[NS]) {
+__device__ __forceinline__ void scan_rates(const fsc_selective_scan_args& a, const ScanPlace<L, NS>& w, float (&rate)[NS]) {
 #pragma unroll
     for (int i = 0; i < NS; ++i) {
         const int s = w.sg * NS + i;
-        a2[i] = w.real && s < a.states ? -expf(a.a_log[(long)w.channel * a.states + s]) * kLog2e : 0.f;
+        rate[i] = w.real && s < a.states ? -expf(a.a_log[(long)w.channel * a.states + s]) : 0.f;
     }
 }
 

@@ -12,17 +12,15 @@ using namespace fsc;
 template <typename T, int L, int NS, bool ENDS>
 __global__ __launch_bounds__(256) void scan_fwd_kernel(fsc_selective_scan_args a, ScanPlan p, float* ends, float* end_deltas) {
     using Place = ScanPlace<L, NS>;
-    constexpr int CB = Place::CB, E = Place::E, SP = Place::SP, ROWS = Place::ROWS;
+    constexpr int CB = Place::CB, E = Place::E, SP = Place::SP;
     __shared__ __align__(16) float s_delta[CB][kPad], s_du[CB][kPad], s_y[ENDS ? 1 : CB][kPad];
     __shared__ __align__(16) float s_b[kTile][SP], s_c[ENDS ? 1 : kTile][SP];
-    const Place w(a, p);
+    int len;
+    const Place w(a, p, len);
     if (ENDS && w.segment == p.segments - 1) return;
-    const int len = scan_frames(a, w.n);
-    const int first = w.segment * p.segment_tiles;
-    const int last = first + p.segment_tiles < p.tiles ? first + p.segment_tiles : p.tiles;
 
-    float a2[NS], h[NS], sum = 0.f;
-    scan_rates(a, w, a2);
+    float rate[NS], h[NS], sum = 0.f;
+    scan_rates(a, w, rate);
     scan_state(a, w, ENDS ? nullptr : a.initial, h);
     if constexpr (!ENDS) {
         for (int q = 0; q < w.segment; ++q) {
@@ -30,56 +28,40 @@ __global__ __launch_bounds__(256) void scan_fwd_kernel(fsc_selective_scan_args a
             float e[NS];
             load_row<NS>(ends + w.end(p, q), true, NS, e);
 #pragma unroll
-            for (int i = 0; i < NS; ++i) h[i] = fmaf(__builtin_amdgcn_exp2f(a2[i] * ds), h[i], e[i]);
+            for (int i = 0; i < NS; ++i) h[i] = fmaf(__builtin_amdgcn_exp2f(rate[i] * ds), h[i], e[i]);
         }
     }
     float bias[E], skip[E];
 #pragma unroll
     for (int i = 0; i < E; ++i) {
-        bias[i] = a.dt_bias != nullptr && i < w.he ? a.dt_bias[w.c0 + w.ce + i] : 0.f;
+        bias[i] = a.dt_bias != nullptr && i < w.he ? a.dt_bias[w.c0 + w.ce + i] * kLog2e : 0.f;
         skip[i] = !ENDS && a.d != nullptr && i < w.he ? a.d[w.c0 + w.ce + i] : 0.f;
     }
-    const bool wide = p.wide && w.he == E;
-    const long c = w.c0 + w.ce;
-    float u_next[E], dt_next[E], z_next[E], b_next[ROWS], c_next[ROWS];
+    const ScanFrames<T, L, NS> u_rows(w, a.u, a.u_batch, a.u_time), dt_rows(w, a.dt, a.dt_batch, a.dt_time), z_rows(w, a.z, a.z_batch, a.z_time);
+    ScanRows<T, L, NS> b_rows(w, a.b, a.b_batch, a.b_time, a.b_group, a.states), c_rows(w, a.c, a.c_batch, a.c_time, a.c_group, a.states);
+    Pack<T, E> u_next, dt_next, z_next;
     auto fetch = [&](int tile) {
-        const int t = tile * kTile + w.te;
-        const int he = t < len ? w.he : 0;
-        const bool go = wide && t < len;
-        load_row<E>(reinterpret_cast<const T*>(a.u) + w.n * a.u_batch + t * a.u_time + c, go, he, u_next);
-        load_row<E>(reinterpret_cast<const T*>(a.dt) + w.n * a.dt_batch + t * a.dt_time + c, go, he, dt_next);
-        if (!ENDS && a.z != nullptr) load_row<E>(reinterpret_cast<const T*>(a.z) + w.n * a.z_batch + t * a.z_time + c, go, he, z_next);
-#pragma unroll
-        for (int j = 0; j < ROWS; ++j) {
-            const int tr = tile * kTile + w.bc_row(j), s = w.bc_state(j);
-            const bool there = w.bc_mine(j) && tr < len && s < a.states;
-            b_next[j] = there ? (float)reinterpret_cast<const T*>(a.b)[w.n * a.b_batch + tr * a.b_time + w.group * a.b_group + s] : 0.f;
-            if (!ENDS)
-                c_next[j] = there ? (float)reinterpret_cast<const T*>(a.c)[w.n * a.c_batch + tr * a.c_time + w.group * a.c_group + s] : 0.f;
-        }
+        u_rows.fetch(w, tile, len, u_next);
+        dt_rows.fetch(w, tile, len, dt_next);
+        if (!ENDS && a.z != nullptr) z_rows.fetch(w, tile, len, z_next);
+        b_rows.fetch(w, tile, len);
+        if (!ENDS) c_rows.fetch(w, tile, len);
     };
-    const int work_end = tiles_with(len) < last ? tiles_with(len) : last;      // tiles behind it hold no frame
-    if (first < work_end) fetch(first);
-    for (int tile = first; tile < work_end; ++tile) {
+    if (w.first < w.work_end) fetch(w.first);
+    for (int tile = w.first; tile < w.work_end; ++tile) {
         const int t = tile * kTile + w.te;
-        float u[E], z[E];
+        float raw[E], delta[E];
+        time_steps(dt_next, bias, a.softplus, t < len, raw, delta);
+        const Pack<T, E> u_now = u_next, z_now = z_next;
 #pragma unroll
         for (int i = 0; i < E; ++i) {
-            u[i] = u_next[i];
-            z[i] = ENDS ? 0.f : z_next[i];
-            const float raw = dt_next[i] + bias[i];
-            const float delta = t < len ? (a.softplus ? softplus_fast(raw) : raw) : 0.f;
-            s_delta[w.ce + i][w.te] = delta;
-            s_du[w.ce + i][w.te] = delta * u[i];
+            s_delta[w.lds_row(i)][w.te] = delta[i];
+            s_du[w.lds_row(i)][w.te] = t < len ? delta[i] * (float)u_now.v[i] : 0.f;
         }
-#pragma unroll
-        for (int j = 0; j < ROWS; ++j)
-            if (w.bc_mine(j)) {
-                s_b[w.bc_row(j)][w.bc_state(j)] = b_next[j];
-                if (!ENDS) s_c[w.bc_row(j)][w.bc_state(j)] = c_next[j];
-            }
+        b_rows.stage(w, s_b, tile, len, a.states, kLn2);
+        if constexpr (!ENDS) c_rows.stage(w, s_c, tile, len, a.states, 1.0f);
         __syncthreads();
-        if (tile + 1 < work_end) fetch(tile + 1);
+        if (tile + 1 < w.work_end) fetch(tile + 1);
         if (!ENDS && a.checkpoints != nullptr) store_row<NS>(a.checkpoints + w.kept(p, tile), true, NS, h);
 #pragma unroll
         for (int q = 0; q < kTile / 4; ++q) {
@@ -94,16 +76,14 @@ __global__ __launch_bounds__(256) void scan_fwd_kernel(fsc_selective_scan_args a
                 float v = 0.f;
 #pragma unroll
                 for (int i = 0; i < NS; ++i) {
-                    h[i] = fmaf(__builtin_amdgcn_exp2f(dl[j] * a2[i]), h[i], du[j] * b[i]);
+                    h[i] = fmaf(__builtin_amdgcn_exp2f(dl[j] * rate[i]), h[i], du[j] * b[i]);
                     if constexpr (!ENDS) v = fmaf(cc[i], h[i], v);
                 }
                 if constexpr (ENDS) sum += dl[j];
                 else y[j] = group_sum<L>(v);
             }
             if constexpr (!ENDS) {
-                const int k = w.sg & 3;
-                const float mine = k == 0 ? y[0] : k == 1 ? y[1] : k == 2 ? y[2] : y[3];
-                if (w.sg < 4) s_y[w.ch][4 * q + k] = mine;
+                if (L == 4 || w.sg < 4) s_y[w.ch][4 * q + (w.sg & 3)] = pick4(y[0], y[1], y[2], y[3], w.sg);
             }
         }
         __syncthreads();
@@ -111,12 +91,14 @@ __global__ __launch_bounds__(256) void scan_fwd_kernel(fsc_selective_scan_args a
             if (t < a.length) {
                 float y[E];
 #pragma unroll
-                for (int i = 0; i < E; ++i) {
-                    float v = fmaf(skip[i], u[i], s_y[w.ce + i][w.te]);
-                    if (a.z != nullptr) v *= z[i] * sigmoid_fast(z[i]);
-                    y[i] = t < len ? v : 0.f;
+                for (int i = 0; i < E; ++i) y[i] = fmaf(skip[i], (float)u_now.v[i], s_y[w.lds_row(i)][w.te]);
+                if (a.z != nullptr) {
+#pragma unroll
+                    for (int i = 0; i < E; ++i) y[i] *= (float)z_now.v[i] * sigmoid_fast((float)z_now.v[i]);
                 }
-                store_row<E>(reinterpret_cast<T*>(a.y) + ((long)w.n * a.length + t) * a.channels + c, wide, w.he, y);
+#pragma unroll
+                for (int i = 0; i < E; ++i) y[i] = t < len ? y[i] : 0.f;
+                store_row<E>(scan_out<T>(a, w, a.y, tile), w.whole, w.he, y);
             }
         }
     }
@@ -124,10 +106,9 @@ __global__ __launch_bounds__(256) void scan_fwd_kernel(fsc_selective_scan_args a
         store_row<NS>(ends + w.end(p, w.segment), true, NS, h);
         if (w.sg == 0) end_deltas[w.end_delta(p, w.segment)] = sum;
     } else {
-        for (int tile = work_end > first ? work_end : first; tile < last; ++tile) {
-            const int t = tile * kTile + w.te;
+        for (int tile = w.zero_first; tile < w.zero_end; ++tile) {
             float zero[E] = {};
-            if (t < a.length) store_row<E>(reinterpret_cast<T*>(a.y) + ((long)w.n * a.length + t) * a.channels + c, wide, w.he, zero);
+            if (tile * kTile + w.te < a.length) store_row<E>(scan_out<T>(a, w, a.y, tile), w.whole, w.he, zero);
         }
         if (a.final != nullptr && w.segment == p.segments - 1 && w.real) {
 #pragma unroll
@@ -139,40 +120,61 @@ __global__ __launch_bounds__(256) void scan_fwd_kernel(fsc_selective_scan_args a
     }
 }
 
-// One frame.  Bound: the state, read and written once; L lanes a channel as in the scan, four states a lane in one 16-byte access.
-template <typename T, int L, int NS>
-__global__ __launch_bounds__(256) void scan_step_kernel(fsc_selective_scan_args a, int wide) {
-    const long slot = (long)blockIdx.x * (256 / L) + threadIdx.x / L;
-    const int sg = threadIdx.x % L;
-    const bool real = slot < (long)a.batch * a.channels;
-    const long n = real ? slot / a.channels : 0;
-    const int c = real ? (int)(slot % a.channels) : 0, group = c / (a.channels / a.groups);
-    const int s0 = sg * NS, have = a.states - s0 < 0 || !real ? 0 : a.states - s0 < NS ? a.states - s0 : NS;
-    float* state = a.final + (n * a.channels + c) * a.states + s0;
-    float h[NS], al[NS], b[NS], cc[NS];
+// One frame.  Bound: the state, read and written once, in 16-byte accesses; L lanes a channel as in the scan.  A workgroup takes R x CB
+// channels of one sequence, each thread R of them with all their loads in flight and one read of B and C.
+template <typename T, int L, int NS, int R>
+__global__ __launch_bounds__(256) void scan_step_kernel(fsc_selective_scan_args a, int group_channels, int group_blocks, int wide) {
+    constexpr int CB = 256 / L;
+    const int blocks = a.groups * group_blocks;
+    const long n = blockIdx.x / blocks;
+    const int block = blockIdx.x % blocks, group = block / group_blocks, first = (block % group_blocks) * (CB * R);
+    const int sg = threadIdx.x % L, s0 = sg * NS;
+    const int have = a.states - s0 < 0 ? 0 : a.states - s0 < NS ? a.states - s0 : NS;
     const bool go = wide && have == NS;
-    load_row<NS>(state, go, have, h);
-    load_row<NS>(a.a_log + (long)c * a.states + s0, go, have, al);
+    float b[NS], cc[NS], h[R][NS], al[R][NS], u[R], dt[R], z[R];
+    int c[R];
+    bool real[R];
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+        const int in_group = first + r * CB + threadIdx.x / L;
+        real[r] = in_group < group_channels;
+        c[r] = group * group_channels + (real[r] ? in_group : 0);
+        const float* state = a.final + (n * a.channels + c[r]) * a.states + s0;
+        const float* rate = a.a_log + (long)c[r] * a.states + s0;
+        if (go) {
+            const Pack<float, NS> hv = load_pack<float, NS>(state), av = load_pack<float, NS>(rate);
+#pragma unroll
+            for (int i = 0; i < NS; ++i) {
+                h[r][i] = hv.v[i];
+                al[r][i] = av.v[i];
+            }
+        } else {
+            load_row<NS>(state, false, have, h[r]);
+            load_row<NS>(rate, false, have, al[r]);
+        }
+        u[r] = (float)reinterpret_cast<const T*>(a.u)[n * a.u_batch + c[r]];
+        dt[r] = ((float)reinterpret_cast<const T*>(a.dt)[n * a.dt_batch + c[r]] + (a.dt_bias != nullptr ? a.dt_bias[c[r]] : 0.f)) * kLog2e;
+        z[r] = a.z != nullptr ? (float)reinterpret_cast<const T*>(a.z)[n * a.z_batch + c[r]] : 0.f;
+    }
     load_row<NS>(reinterpret_cast<const T*>(a.b) + n * a.b_batch + group * a.b_group + s0, false, have, b);
     load_row<NS>(reinterpret_cast<const T*>(a.c) + n * a.c_batch + group * a.c_group + s0, false, have, cc);
-    const float u = (float)reinterpret_cast<const T*>(a.u)[n * a.u_batch + c];
-    const float raw = (float)reinterpret_cast<const T*>(a.dt)[n * a.dt_batch + c] + (a.dt_bias != nullptr ? a.dt_bias[c] : 0.f);
-    const float delta = a.softplus ? softplus_fast(raw) : raw;
-    float v = 0.f;
 #pragma unroll
-    for (int i = 0; i < NS; ++i) {
-        h[i] = fmaf(__builtin_amdgcn_exp2f(delta * (-__expf(al[i]) * kLog2e)), h[i], delta * u * b[i]);
-        if (i < have) v = fmaf(cc[i], h[i], v);
-    }
-    store_row<NS>(state, go, have, h);
-    v = group_sum<L>(v);
-    if (sg == 0 && real) {
-        if (a.d != nullptr) v = fmaf(a.d[c], u, v);
-        if (a.z != nullptr) {
-            const float z = (float)reinterpret_cast<const T*>(a.z)[n * a.z_batch + c];
-            v *= z * sigmoid_fast(z);
+    for (int r = 0; r < R; ++r) {
+        const float delta = a.softplus ? softplus2(dt[r]) : dt[r];
+        float v = 0.f;
+#pragma unroll
+        for (int i = 0; i < NS; ++i) {
+            h[r][i] = fmaf(__builtin_amdgcn_exp2f(delta * -__expf(al[r][i])), h[r][i], delta * kLn2 * u[r] * b[i]);
+            if (i < have) v = fmaf(cc[i], h[r][i], v);
         }
-        reinterpret_cast<T*>(a.y)[slot] = (T)v;
+        v = group_sum<L>(v);
+        if (!real[r]) continue;
+        store_row<NS>(a.final + (n * a.channels + c[r]) * a.states + s0, go, have, h[r]);
+        if (sg == 0) {
+            if (a.d != nullptr) v = fmaf(a.d[c[r]], u[r], v);
+            if (a.z != nullptr) v *= z[r] * sigmoid_fast(z[r]);
+            reinterpret_cast<T*>(a.y)[n * a.channels + c[r]] = (T)v;
+        }
     }
 }
 
@@ -219,13 +221,18 @@ int fsc_selective_scan_step(const fsc_selective_scan_args* args_host, fsc_stream
     FSC_CHECK_ARG(a.u && a.dt && a.b && a.c && a.y && a.final, "fsc_selective_scan_step: null u, dt, b, c, y or state");
     const ScanPlan p = scan_plan(a);
     const int wide = a.states % p.per_lane == 0 && aligned(a.final, 4 * p.per_lane) && aligned(a.a_log, 4 * p.per_lane);
-    const long slots = (long)a.batch * a.channels;
-    const dim3 grid((unsigned)ceil_div(slots, p.channels_block));
+    // four channels a thread where that still leaves two workgroups a CU, else one
+    const long fours = (long)a.batch * a.groups * ceil_div(p.group_channels, 4 * p.channels_block);
+    const int r = fours >= 512 ? 4 : 1, group_blocks = ceil_div(p.group_channels, r * p.channels_block);
+    const dim3 grid((unsigned)((long)a.batch * a.groups * group_blocks));
     auto typed = [&](auto type) {
         using T = decltype(type);
         with_scan_shape(p, [&](auto lanes, auto per) {
-            hipLaunchKernelGGL((scan_step_kernel<T, decltype(lanes)::value, decltype(per)::value>), grid, dim3(256), 0, as_stream(stream), a,
-                               wide);
+            constexpr int L = decltype(lanes)::value, NS = decltype(per)::value;
+            if (r == 4)
+                hipLaunchKernelGGL((scan_step_kernel<T, L, NS, 4>), grid, dim3(256), 0, as_stream(stream), a, p.group_channels, group_blocks, wide);
+            else
+                hipLaunchKernelGGL((scan_step_kernel<T, L, NS, 1>), grid, dim3(256), 0, as_stream(stream), a, p.group_channels, group_blocks, wide);
         });
     };
     FSC_WITH_DTYPE(a.dtype, typed);

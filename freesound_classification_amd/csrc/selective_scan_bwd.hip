@@ -32,43 +32,45 @@ struct Carve {
 template <typename T, int L, int NS>
 __global__ __launch_bounds__(256) void scan_bwd_ends_kernel(fsc_selective_scan_args a, ScanPlan p, float* ends, float* end_deltas) {
     using Place = ScanPlace<L, NS>;
-    constexpr int CB = Place::CB, E = Place::E, SP = Place::SP, ROWS = Place::ROWS;
+    constexpr int CB = Place::CB, E = Place::E, SP = Place::SP;
     __shared__ __align__(16) float s_delta[CB][kPad], s_dyy[CB][kPad], s_c[kTile][SP];
-    const Place w(a, p);
+    int len;
+    const Place w(a, p, len);
     if (w.segment == 0) return;
-    const int len = scan_frames(a, w.n);
-    const int first = w.segment * p.segment_tiles;
-    const int last = first + p.segment_tiles < p.tiles ? first + p.segment_tiles : p.tiles;
-    float a2[NS], e[NS] = {}, sum = 0.f;
-    scan_rates(a, w, a2);
+    float rate[NS], e[NS] = {}, sum = 0.f;
+    scan_rates(a, w, rate);
     float bias[E];
 #pragma unroll
-    for (int i = 0; i < E; ++i) bias[i] = a.dt_bias != nullptr && i < w.he ? a.dt_bias[w.c0 + w.ce + i] : 0.f;
-    const bool wide = p.wide && w.he == E;
-    const long c = w.c0 + w.ce;
-    const int work_end = tiles_with(len) < last ? tiles_with(len) : last;
-    for (int tile = work_end - 1; tile >= first; --tile) {
-        const int t = tile * kTile + w.te, he = t < len ? w.he : 0;
-        const bool go = wide && t < len;
-        float dt[E], z[E], dy[E];
-        load_row<E>(reinterpret_cast<const T*>(a.dt) + w.n * a.dt_batch + t * a.dt_time + c, go, he, dt);
-        load_row<E>(reinterpret_cast<const T*>(a.dy) + w.n * a.dy_batch + t * a.dy_time + c, go && a.dy != nullptr, a.dy != nullptr ? he : 0, dy);
-        if (a.z != nullptr) load_row<E>(reinterpret_cast<const T*>(a.z) + w.n * a.z_batch + t * a.z_time + c, go, he, z);
+    for (int i = 0; i < E; ++i) bias[i] = a.dt_bias != nullptr && i < w.he ? a.dt_bias[w.c0 + w.ce + i] * kLog2e : 0.f;
+    const ScanFrames<T, L, NS> dt_rows(w, a.dt, a.dt_batch, a.dt_time), z_rows(w, a.z, a.z_batch, a.z_time), dy_rows(w, a.dy, a.dy_batch, a.dy_time);
+    ScanRows<T, L, NS> c_rows(w, a.c, a.c_batch, a.c_time, a.c_group, a.states);
+    Pack<T, E> dt_next, z_next, dy_next;
+    auto fetch = [&](int tile) {
+        dt_rows.fetch(w, tile, len, dt_next);
+        if (a.dy != nullptr) dy_rows.fetch(w, tile, len, dy_next);
+        if (a.z != nullptr) z_rows.fetch(w, tile, len, z_next);
+        c_rows.fetch(w, tile, len);
+    };
+    if (w.first < w.work_end) fetch(w.work_end - 1);
+    for (int tile = w.work_end - 1; tile >= w.first; --tile) {
+        const int t = tile * kTile + w.te;
         __syncthreads();
+        float raw[E], delta[E], dyy[E];
+        time_steps(dt_next, bias, a.softplus, t < len, raw, delta);
 #pragma unroll
-        for (int i = 0; i < E; ++i) {
-            const float raw = dt[i] + bias[i];
-            s_delta[w.ce + i][w.te] = t < len ? (a.softplus ? softplus_fast(raw) : raw) : 0.f;
-            s_dyy[w.ce + i][w.te] = a.z != nullptr ? dy[i] * (z[i] * sigmoid_fast(z[i])) : dy[i];
+        for (int i = 0; i < E; ++i) dyy[i] = a.dy != nullptr ? (float)dy_next.v[i] : 0.f;
+        if (a.z != nullptr) {
+#pragma unroll
+            for (int i = 0; i < E; ++i) dyy[i] *= (float)z_next.v[i] * sigmoid_fast((float)z_next.v[i]);
         }
 #pragma unroll
-        for (int j = 0; j < ROWS; ++j)
-            if (w.bc_mine(j)) {
-                const int tr = tile * kTile + w.bc_row(j), s = w.bc_state(j);
-                s_c[w.bc_row(j)][s] =
-                    tr < len && s < a.states ? (float)reinterpret_cast<const T*>(a.c)[w.n * a.c_batch + tr * a.c_time + w.group * a.c_group + s] : 0.f;
-            }
+        for (int i = 0; i < E; ++i) {
+            s_delta[w.lds_row(i)][w.te] = delta[i];
+            s_dyy[w.lds_row(i)][w.te] = t < len ? dyy[i] : 0.f;
+        }
+        c_rows.stage(w, s_c, tile, len, a.states, 1.0f);
         __syncthreads();
+        if (tile > w.first) fetch(tile - 1);
 #pragma unroll
         for (int q = kTile / 4 - 1; q >= 0; --q) {
             float dl[4], dyy[4];
@@ -79,7 +81,7 @@ __global__ __launch_bounds__(256) void scan_bwd_ends_kernel(fsc_selective_scan_a
                 float cc[NS];
                 load_row<NS>(&s_c[4 * q + j][w.sg * NS], true, NS, cc);
 #pragma unroll
-                for (int i = 0; i < NS; ++i) e[i] = __builtin_amdgcn_exp2f(dl[j] * a2[i]) * fmaf(cc[i], dyy[j], e[i]);
+                for (int i = 0; i < NS; ++i) e[i] = __builtin_amdgcn_exp2f(dl[j] * rate[i]) * fmaf(cc[i], dyy[j], e[i]);
                 sum += dl[j];
             }
         }
@@ -120,97 +122,94 @@ __device__ __forceinline__ void channel_sums(float (&v)[2 * NS], int lane) {
 template <typename T, int L, int NS>
 __global__ __launch_bounds__(256, 2) void scan_bwd_kernel(fsc_selective_scan_args a, ScanPlan p, Carve at) {
     using Place = ScanPlace<L, NS>;
-    constexpr int CB = Place::CB, E = Place::E, SP = Place::SP, ROWS = Place::ROWS;
-    __shared__ __align__(16) float s_delta[CB][kPad], s_du[CB][kPad], s_dyy[CB][kPad], s_yh[CB][kPad];
+    constexpr int CB = Place::CB, E = Place::E, SP = Place::SP;
+    __shared__ __align__(16) float s_delta[CB][kPad], s_du[CB][kPad], s_dyy[CB][kPad], s_yh[CB][kPad], s_gb[CB][kPad], s_ga[CB][kPad];
+    __shared__ __align__(16) float s_sig[256][E], s_gz[256][E];       // a thread's own, out of its registers while it scans
     __shared__ __align__(16) float s_b[kTile][SP], s_c[kTile][SP];
     __shared__ __align__(16) float s_red[kTile][4][2][SP];
     float* ws = reinterpret_cast<float*>(a.workspace);
-    const Place w(a, p);
+    int len;
+    const Place w(a, p, len);
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int len = scan_frames(a, w.n);
-    const int first = w.segment * p.segment_tiles;
-    const int last = first + p.segment_tiles < p.tiles ? first + p.segment_tiles : p.tiles;
 
-    float a2[NS], e[NS], da[NS] = {};              // e: exp(delta_{t+1} A) G_{t+1}, what reaches h_t from behind
-    scan_rates(a, w, a2);
+    float rate[NS], e[NS], da[NS] = {};              // e: exp(delta_{t+1} A) G_{t+1}, what reaches h_t from behind
+    scan_rates(a, w, rate);
     scan_state(a, w, a.dfinal, e);
     for (int q = p.segments - 1; q > w.segment; --q) {
         const float ds = ws[at.end_deltas + w.end_delta(p, q)];
         float more[NS];
         load_row<NS>(ws + at.ends + w.end(p, q), true, NS, more);
 #pragma unroll
-        for (int i = 0; i < NS; ++i) e[i] = fmaf(__builtin_amdgcn_exp2f(a2[i] * ds), e[i], more[i]);
+        for (int i = 0; i < NS; ++i) e[i] = fmaf(__builtin_amdgcn_exp2f(rate[i] * ds), e[i], more[i]);
     }
     float bias[E], skip[E], dskip[E] = {}, dbias[E] = {};
 #pragma unroll
     for (int i = 0; i < E; ++i) {
-        bias[i] = a.dt_bias != nullptr && i < w.he ? a.dt_bias[w.c0 + w.ce + i] : 0.f;
+        bias[i] = a.dt_bias != nullptr && i < w.he ? a.dt_bias[w.c0 + w.ce + i] * kLog2e : 0.f;
         skip[i] = a.d != nullptr && i < w.he ? a.d[w.c0 + w.ce + i] : 0.f;
     }
-    const bool wide = p.wide && w.he == E;
-    const long c = w.c0 + w.ce;
-    float u_next[E], dt_next[E], z_next[E], dy_next[E], b_next[ROWS], c_next[ROWS], h_next[NS];
+    const ScanFrames<T, L, NS> u_rows(w, a.u, a.u_batch, a.u_time), dt_rows(w, a.dt, a.dt_batch, a.dt_time), z_rows(w, a.z, a.z_batch, a.z_time),
+        dy_rows(w, a.dy, a.dy_batch, a.dy_time);
+    ScanRows<T, L, NS> b_rows(w, a.b, a.b_batch, a.b_time, a.b_group, a.states), c_rows(w, a.c, a.c_batch, a.c_time, a.c_group, a.states);
+    Pack<T, E> u_next, dt_next, z_next, dy_next;
+    Pack<float, NS> h_next;
     auto fetch = [&](int tile) {
-        const int t = tile * kTile + w.te;
-        const int he = t < len ? w.he : 0;
-        const bool go = wide && t < len;
-        load_row<E>(reinterpret_cast<const T*>(a.u) + w.n * a.u_batch + t * a.u_time + c, go, he, u_next);
-        load_row<E>(reinterpret_cast<const T*>(a.dt) + w.n * a.dt_batch + t * a.dt_time + c, go, he, dt_next);
-        if (a.z != nullptr) load_row<E>(reinterpret_cast<const T*>(a.z) + w.n * a.z_batch + t * a.z_time + c, go, he, z_next);
-        load_row<E>(reinterpret_cast<const T*>(a.dy) + w.n * a.dy_batch + t * a.dy_time + c, go && a.dy != nullptr, a.dy != nullptr ? he : 0, dy_next);
-#pragma unroll
-        for (int j = 0; j < ROWS; ++j) {
-            const int tr = tile * kTile + w.bc_row(j), s = w.bc_state(j);
-            const bool there = w.bc_mine(j) && tr < len && s < a.states;
-            b_next[j] = there ? (float)reinterpret_cast<const T*>(a.b)[w.n * a.b_batch + tr * a.b_time + w.group * a.b_group + s] : 0.f;
-            c_next[j] = there ? (float)reinterpret_cast<const T*>(a.c)[w.n * a.c_batch + tr * a.c_time + w.group * a.c_group + s] : 0.f;
-        }
-        load_row<NS>(a.checkpoints + w.kept(p, tile), true, NS, h_next);
+        u_rows.fetch(w, tile, len, u_next);
+        dt_rows.fetch(w, tile, len, dt_next);
+        if (a.dy != nullptr) dy_rows.fetch(w, tile, len, dy_next);
+        if (a.z != nullptr) z_rows.fetch(w, tile, len, z_next);
+        b_rows.fetch(w, tile, len);
+        c_rows.fetch(w, tile, len);
+        h_next = load_pack<float, NS>(a.checkpoints + w.kept(p, tile));
     };
-    const int work_end = tiles_with(len) < last ? tiles_with(len) : last;      // tiles behind it hold no frame
-    for (int tile = work_end > first ? work_end : first; tile < last; ++tile) {
-        const int t = tile * kTile + w.te;
+    for (int tile = w.zero_first; tile < w.zero_end; ++tile) {
         float zero[E] = {};
-        if (t < a.length) {
-            const long o = ((long)w.n * a.length + t) * a.channels + c;
-            store_row<E>(reinterpret_cast<T*>(a.du) + o, wide, w.he, zero);
-            store_row<E>(reinterpret_cast<T*>(a.ddt) + o, wide, w.he, zero);
-            if (a.z != nullptr) store_row<E>(reinterpret_cast<T*>(a.dz) + o, wide, w.he, zero);
+        if (tile * kTile + w.te < a.length) {
+            store_row<E>(scan_out<T>(a, w, a.du, tile), w.whole, w.he, zero);
+            store_row<E>(scan_out<T>(a, w, a.ddt, tile), w.whole, w.he, zero);
+            if (a.z != nullptr) store_row<E>(scan_out<T>(a, w, a.dz, tile), w.whole, w.he, zero);
         }
-        for (int j = threadIdx.x; j < kTile * 2 * SP; j += 256)
-            ws[at.rows + (((long)w.n * p.blocks + w.block) * p.tiles + tile) * (kTile * 2 * SP) + j] = 0.f;
+        for (int j = threadIdx.x; j < kTile * 2 * SP; j += 256) ws[at.rows + w.rows(p, tile) + j] = 0.f;
     }
-    if (first < work_end) fetch(work_end - 1);
-    for (int tile = work_end - 1; tile >= first; --tile) {
+    if (w.first < w.work_end) fetch(w.work_end - 1);
+    for (int tile = w.work_end - 1; tile >= w.first; --tile) {
         const int t = tile * kTile + w.te;
-        float u[E], delta[E], sig[E], gz[E], dyy[E], h[NS], hp[kTile][NS], ex[kTile][NS];
+        const Pack<T, E> u_now = u_next;
+        float raw[E], delta[E], dyy[E], sig[E], gz[E], h[NS], hp[kTile][NS], ex[kTile][NS];
+        time_steps(dt_next, bias, a.softplus, t < len, raw, delta);
 #pragma unroll
         for (int i = 0; i < E; ++i) {
-            u[i] = u_next[i];
-            const float raw = dt_next[i] + bias[i];
-            delta[i] = t < len ? (a.softplus ? softplus_fast(raw) : raw) : 0.f;
-            sig[i] = t < len ? (a.softplus ? sigmoid_fast(raw) : 1.0f) : 0.f;
-            dyy[i] = dy_next[i];
+            dyy[i] = t < len && i < w.he && a.dy != nullptr ? (float)dy_next.v[i] : 0.f;
+            sig[i] = 1.0f;
             gz[i] = 0.f;
-            if (a.z != nullptr) {
-                const float s = sigmoid_fast(z_next[i]);
-                gz[i] = dy_next[i] * (s * fmaf(z_next[i], 1.0f - s, 1.0f));
-                dyy[i] = dy_next[i] * (z_next[i] * s);
+        }
+        if (a.softplus) {
+#pragma unroll
+            for (int i = 0; i < E; ++i) sig[i] = sigmoid2(raw[i]);
+        }
+        if (a.z != nullptr) {
+#pragma unroll
+            for (int i = 0; i < E; ++i) {
+                const float z = t < len ? (float)z_next.v[i] : 0.f, s = sigmoid_fast(z), zs = z * s;
+                gz[i] = dyy[i] * (fmaf(-zs, s, zs) + s);
+                dyy[i] *= zs;
             }
-            s_delta[w.ce + i][w.te] = delta[i];
-            s_du[w.ce + i][w.te] = delta[i] * u[i];
-            s_dyy[w.ce + i][w.te] = dyy[i];
         }
 #pragma unroll
-        for (int j = 0; j < ROWS; ++j)
-            if (w.bc_mine(j)) {
-                s_b[w.bc_row(j)][w.bc_state(j)] = b_next[j];
-                s_c[w.bc_row(j)][w.bc_state(j)] = c_next[j];
-            }
+        for (int i = 0; i < E; ++i) {
+            s_delta[w.lds_row(i)][w.te] = delta[i];
+            // (a channel that does not exist must not enter the sums over channels)
+            s_du[w.lds_row(i)][w.te] = t < len && i < w.he ? delta[i] * (float)u_now.v[i] : 0.f;
+            s_dyy[w.lds_row(i)][w.te] = dyy[i];
+        }
+        store_row<E>(s_sig[threadIdx.x], true, E, sig);
+        store_row<E>(s_gz[threadIdx.x], true, E, gz);
+        b_rows.stage(w, s_b, tile, len, a.states, kLn2);
+        c_rows.stage(w, s_c, tile, len, a.states, 1.0f);
 #pragma unroll
-        for (int i = 0; i < NS; ++i) h[i] = h_next[i];
+        for (int i = 0; i < NS; ++i) h[i] = h_next.v[i];
         __syncthreads();
-        if (tile > first) fetch(tile - 1);
+        if (tile > w.first) fetch(tile - 1);
 #pragma unroll
         for (int q = 0; q < kTile / 4; ++q) {
             float dl[4], du[4], y[4];
@@ -223,16 +222,15 @@ __global__ __launch_bounds__(256, 2) void scan_bwd_kernel(fsc_selective_scan_arg
                 load_row<NS>(&s_c[4 * q + j][w.sg * NS], true, NS, cc);
 #pragma unroll
                 for (int i = 0; i < NS; ++i) {
-                    ex[4 * q + j][i] = __builtin_amdgcn_exp2f(dl[j] * a2[i]);
+                    ex[4 * q + j][i] = __builtin_amdgcn_exp2f(dl[j] * rate[i]);
                     hp[4 * q + j][i] = h[i];
                     h[i] = fmaf(ex[4 * q + j][i], h[i], du[j] * b[i]);
                     v = fmaf(cc[i], h[i], v);
                 }
                 y[j] = group_sum<L>(v);
             }
-            const int k = w.sg & 3;
-            const float mine = k == 0 ? y[0] : k == 1 ? y[1] : k == 2 ? y[2] : y[3];
-            if (w.sg < 4) s_yh[w.ch][4 * q + k] = mine;
+            if (L == 4 || w.sg < 4) s_yh[w.ch][4 * q + (w.sg & 3)] = pick4(y[0], y[1], y[2], y[3], w.sg);
+            __builtin_amdgcn_sched_barrier(0);        // (else the reads of later frames are hoisted until registers spill)
         }
 #pragma unroll
         for (int q = kTile / 4 - 1; q >= 0; --q) {
@@ -252,10 +250,10 @@ __global__ __launch_bounds__(256, 2) void scan_bwd_kernel(fsc_selective_scan_arg
                     v[i] = g * du[j];
                     v[NS + i] = h[i] * dyy4[j];
                     gb = fmaf(g, b[i], gb);
-                    const float gx = g * (ex[k][i] * hp[k][i]);
-                    da[i] = fmaf(gx, dl[j], da[i]);
-                    ga = fmaf(gx, a2[i], ga);
                     e[i] = ex[k][i] * g;
+                    const float gx = e[i] * hp[k][i];
+                    da[i] = fmaf(gx, dl[j], da[i]);
+                    ga = fmaf(gx, rate[i], ga);
                     h[i] = hp[k][i];
                 }
                 gb4[j] = group_sum<L>(gb);
@@ -270,38 +268,36 @@ __global__ __launch_bounds__(256, 2) void scan_bwd_kernel(fsc_selective_scan_arg
                     for (int i = 0; i < kept; ++i) s_red[k][wave][half][s + i] = v[i];
                 }
             }
-            // (the four frames' delta and delta u have been read by all lanes of this channel: their places take the sums)
-            const int k = w.sg & 3;
-            const float mine_b = k == 0 ? gb4[0] : k == 1 ? gb4[1] : k == 2 ? gb4[2] : gb4[3];
-            const float mine_a = k == 0 ? ga4[0] : k == 1 ? ga4[1] : k == 2 ? ga4[2] : ga4[3];
-            if (w.sg < 4) {
-                s_du[w.ch][4 * q + k] = mine_b;
-                s_delta[w.ch][4 * q + k] = mine_a;
+            if (L == 4 || w.sg < 4) {
+                s_gb[w.ch][4 * q + (w.sg & 3)] = pick4(gb4[0], gb4[1], gb4[2], gb4[3], w.sg);
+                s_ga[w.ch][4 * q + (w.sg & 3)] = pick4(ga4[0], ga4[1], ga4[2], ga4[3], w.sg);
             }
+            __builtin_amdgcn_sched_barrier(0);
         }
         __syncthreads();
         for (int j = threadIdx.x; j < kTile * 2 * SP; j += 256) {
             const int k = j / (2 * SP), rest = j % (2 * SP);
             const float* r = &s_red[k][0][0][rest];
-            ws[at.rows + (((long)w.n * p.blocks + w.block) * p.tiles + tile) * (kTile * 2 * SP) + j] =
-                (r[0] + r[2 * SP]) + (r[4 * SP] + r[6 * SP]);
+            ws[at.rows + w.rows(p, tile) + j] = (r[0] + r[2 * SP]) + (r[4 * SP] + r[6 * SP]);
         }
         if (t < a.length) {
             float du_out[E], ddt_out[E], dz_out[E];
+            load_row<E>(s_sig[threadIdx.x], true, E, sig);
+            load_row<E>(s_gz[threadIdx.x], true, E, gz);
 #pragma unroll
             for (int i = 0; i < E; ++i) {
-                const float gb = s_du[w.ce + i][w.te], ga = s_delta[w.ce + i][w.te] * kLn2;
-                du_out[i] = fmaf(delta[i], gb, skip[i] * dyy[i]);
-                ddt_out[i] = fmaf(u[i], gb, ga) * sig[i];
-                dz_out[i] = gz[i] * fmaf(skip[i], u[i], s_yh[w.ce + i][w.te]);
+                const int r = w.lds_row(i);
+                const float u = t < len ? (float)u_now.v[i] : 0.f, gb = s_gb[r][w.te], ga = s_ga[r][w.te], dyy = s_dyy[r][w.te];
+                du_out[i] = fmaf(s_delta[r][w.te], gb, skip[i] * dyy);          // (B was staged times ln 2, delta over it)
+                ddt_out[i] = fmaf(u * kLog2e, gb, ga) * sig[i];
+                dz_out[i] = gz[i] * fmaf(skip[i], u, s_yh[r][w.te]);
                 if (t >= len) du_out[i] = ddt_out[i] = dz_out[i] = 0.f;
-                dskip[i] = fmaf(dyy[i], u[i], dskip[i]);
+                dskip[i] = fmaf(dyy, u, dskip[i]);
                 dbias[i] += ddt_out[i];
             }
-            const long o = ((long)w.n * a.length + t) * a.channels + c;
-            store_row<E>(reinterpret_cast<T*>(a.du) + o, wide, w.he, du_out);
-            store_row<E>(reinterpret_cast<T*>(a.ddt) + o, wide, w.he, ddt_out);
-            if (a.z != nullptr) store_row<E>(reinterpret_cast<T*>(a.dz) + o, wide, w.he, dz_out);
+            store_row<E>(scan_out<T>(a, w, a.du, tile), w.whole, w.he, du_out);
+            store_row<E>(scan_out<T>(a, w, a.ddt, tile), w.whole, w.he, ddt_out);
+            if (a.z != nullptr) store_row<E>(scan_out<T>(a, w, a.dz, tile), w.whole, w.he, dz_out);
         }
         __syncthreads();
     }
@@ -318,8 +314,8 @@ __global__ __launch_bounds__(256, 2) void scan_bwd_kernel(fsc_selective_scan_arg
     store_row<NS>(mine + ((long)w.block * 256 + threadIdx.x) * NS, true, NS, da);
 #pragma unroll
     for (int i = 0; i < E; ++i) {
-        s_dyy[w.ce + i][w.te] = dskip[i];
-        s_yh[w.ce + i][w.te] = dbias[i];
+        s_dyy[w.lds_row(i)][w.te] = dskip[i];
+        s_yh[w.lds_row(i)][w.te] = dbias[i];
     }
     __syncthreads();
     if (threadIdx.x < CB) {
@@ -334,7 +330,7 @@ __global__ __launch_bounds__(256, 2) void scan_bwd_kernel(fsc_selective_scan_arg
     }
 }
 
-// Joins the partial sums: the first `row_blocks` workgroups dB / dC over the channel blocks of a group, the others (64 columns x 4
+// Joins the partial sums: the first `row_blocks` workgroups dB / dC over the channel blocks of a group, the others (32 columns x 8
 // interleaved shares) the parameters' over sequences and segments.
 template <typename T>
 __global__ __launch_bounds__(256) void scan_bwd_finish_kernel(fsc_selective_scan_args a, ScanPlan p, Carve at, long row_blocks) {
@@ -355,41 +351,41 @@ __global__ __launch_bounds__(256) void scan_bwd_finish_kernel(fsc_selective_scan
             db += from[q * stride];
             dc += from[q * stride + sp];
         }
-        reinterpret_cast<T*>(a.db)[i] = (T)db;
+        reinterpret_cast<T*>(a.db)[i] = (T)(db * kLn2);            // (summed with delta u over ln 2)
         reinterpret_cast<T*>(a.dc)[i] = (T)dc;
         return;
     }
-    __shared__ float red[4][64];
+    __shared__ float red[8][32];
     const long channels = p.padded_channels(), columns = channels * (sp + 2);
-    const long column = ((long)blockIdx.x - row_blocks) * 64 + (threadIdx.x & 63);
-    const int share = threadIdx.x >> 6, count = a.batch * p.segments;
-    float v0 = 0.f, v1 = 0.f;
+    const int k = threadIdx.x & 31, share = threadIdx.x >> 5, count = a.batch * p.segments;
+    const long column = ((long)blockIdx.x - row_blocks) * 32 + k;
+    float v[4] = {};
     if (column < columns) {
         const float* from = ws + at.sums + column;
         int q = share;
-        for (; q + 4 < count; q += 8) {
-            v0 += from[q * columns];
-            v1 += from[(q + 4) * columns];
-        }
-        if (q < count) v0 += from[q * columns];
+        for (; q + 24 < count; q += 32)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) v[i] += from[(q + 8 * i) * columns];
+        for (; q < count; q += 8) v[0] += from[q * columns];
     }
-    red[share][threadIdx.x & 63] = v0 + v1;
+    red[share][k] = (v[0] + v[1]) + (v[2] + v[3]);
     __syncthreads();
     if (share != 0 || column >= columns) return;
-    const int k = threadIdx.x & 63;
-    const float v = (red[0][k] + red[1][k]) + (red[2][k] + red[3][k]);
+    float sum = 0.f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) sum += red[i][k];
     const int cb = p.channels_block;
     const long slot = column < channels * sp ? column / sp : (column - channels * sp) % channels;      // padded channel
-    const int block = (int)(slot / cb), in_group = (block % p.group_blocks) * cb + (int)(slot % cb);
+    const int block = (int)(slot / cb), in_group = (block % p.group_blocks) * cb + channel_of((int)(slot % cb), kTile / p.lanes);
     if (in_group >= p.group_channels) return;
     const long c = (long)(block / p.group_blocks) * p.group_channels + in_group;
     if (column < channels * sp) {
         const int s = (int)(column % sp);
-        if (s < a.states) a.da_log[c * a.states + s] = -expf(a.a_log[c * a.states + s]) * v;           // dA / d a_log = A
+        if (s < a.states) a.da_log[c * a.states + s] = -expf(a.a_log[c * a.states + s]) * kLn2 * sum;         // dA / d a_log = A; delta over ln 2
     } else if (column < channels * (sp + 1)) {
-        if (a.dd != nullptr) a.dd[c] = v;
+        if (a.dd != nullptr) a.dd[c] = sum;
     } else if (a.ddt_bias != nullptr) {
-        a.ddt_bias[c] = v;
+        a.ddt_bias[c] = sum;
     }
 }
 
@@ -418,7 +414,7 @@ int fsc_selective_scan_bwd(const fsc_selective_scan_args* args_host, fsc_stream_
     float* ws = reinterpret_cast<float*>(a.workspace);
     const dim3 grid((unsigned)((long)a.batch * p.blocks * p.segments));
     const long rows = ((long)a.batch * a.length * a.groups * a.states + 255) / 256;
-    const long columns = (p.padded_channels() * (p.padded_states() + 2) + 63) / 64;
+    const long columns = (p.padded_channels() * (p.padded_states() + 2) + 31) / 32;
     FSC_CHECK_ARG(rows + columns < 0x7FFFFFFFL, "fsc_selective_scan_bwd: too large");
     auto typed = [&](auto type) {
         using T = decltype(type);

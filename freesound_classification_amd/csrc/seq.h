@@ -13,11 +13,27 @@ struct alignas(sizeof(T) * V) Pack {
     T v[V];
 };
 
+// The same bytes as one integer word: a wide access must not look like the narrow ones beside it, or the two paths are merged into narrow ones.
+template <int N> struct Word;
+template <> struct Word<2> { typedef uint16_t type; };
+template <> struct Word<4> { typedef uint32_t type; };
+template <> struct Word<8> { typedef uint2 type; };
+template <> struct Word<16> { typedef uint4 type; };
+template <typename T, int V>
+__device__ __forceinline__ Pack<T, V> load_pack(const T* p) {
+    const auto w = *reinterpret_cast<const typename Word<sizeof(T) * V>::type*>(p);
+    return __builtin_bit_cast(Pack<T, V>, w);
+}
+template <typename T, int V>
+__device__ __forceinline__ void store_pack(T* p, const Pack<T, V>& v) {
+    *reinterpret_cast<typename Word<sizeof(T) * V>::type*>(p) = __builtin_bit_cast(typename Word<sizeof(T) * V>::type, v);
+}
+
 // V consecutive values at `p` as floats: one wide load where `wide`, else one by one and only the first `have` (the others are 0).
 template <int V, typename T>
 __device__ __forceinline__ void load_row(const T* p, bool wide, int have, float (&out)[V]) {
     if (wide) {
-        const Pack<T, V> w = *reinterpret_cast<const Pack<T, V>*>(p);
+        const Pack<T, V> w = load_pack<T, V>(p);
 #pragma unroll
         for (int i = 0; i < V; ++i) out[i] = (float)w.v[i];
     } else {
@@ -31,7 +47,7 @@ __device__ __forceinline__ void store_row(T* p, bool wide, int have, const float
         Pack<T, V> w;
 #pragma unroll
         for (int i = 0; i < V; ++i) w.v[i] = (T)in[i];
-        *reinterpret_cast<Pack<T, V>*>(p) = w;
+        store_pack<T, V>(p, w);
     } else {
 #pragma unroll
         for (int i = 0; i < V; ++i)

@@ -37,7 +37,7 @@ def _activation(what, name, t, shape, dtype=None):
     if tuple(t.shape) != tuple(shape):
         _fail(what, "%s has shape %s, expected %s", name, tuple(t.shape), tuple(shape))
     _same_device(what, name, t)
-    if t.shape[-1] > 1 and t.stride(-1) != 1:
+    if (t.shape[-1] > 1 and t.stride(-1) != 1) or (t.dim() > 2 and t.stride(1) > 1 << 26):      # (the kernels step over frames in 32 bits)
         t = t.contiguous()
     return t
 
