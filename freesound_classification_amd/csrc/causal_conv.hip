@@ -1,7 +1,7 @@
 // Short causal convolution along time, one filter of K <= 8 taps a channel, SiLU behind it (the sequence head's local mixing).
 //   pre[t] = bias + sum_k w[k] xin[t + k],  xin = [K - 1 frames before | x];  y = silu(pre)
 // Bound: HBM (two passes over the frames forward, three backward), K multiply-adds and one exponential a value.  So each thread owns
-// 16 bytes of channels (8 backward in 16 bits) and walks a strip of frames with the filter's window in registers: every frame is read
+// four channels and walks a strip of frames with the filter's window in registers: every frame is read
 // once but for the K - 1 at a strip's ends, neighbouring threads read neighbouring channels.  Frames are taken eight at a time, all
 // their loads issued before the first is used.
 // Backward: the strip recomputes pre (cheaper than keeping it) and runs K - 1 frames past its end; dw / db are summed in registers, over
@@ -16,6 +16,7 @@ using fsc::load_row;
 using fsc::store_row;
 
 constexpr int kThreads = 256;
+constexpr int kV = 4;             // channels a thread owns (8 in 16 bits, 16 bytes as well: twice the registers, 146 us for 91 on 4 x 8191 x 2048)
 
 __device__ __forceinline__ float sigmoid_fast(float v) {
     return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(v * -1.44269504088896340736f));
@@ -27,6 +28,7 @@ struct Plan {
     int lanes;         // threads along the channel groups (a power of two), kThreads / lanes rows (sequence, strip) a block
     int rows;          // batch * strips
     int wide;          // every row of V channels is whole and aligned
+    int wide_weights;
 };
 
 __device__ __forceinline__ int frames_of(const fsc_causal_conv_args& a, int n) {
@@ -48,18 +50,81 @@ __device__ __forceinline__ void frame(const fsc_causal_conv_args& a, int n, int 
     }
 }
 
-template <int K, int V>
-__device__ __forceinline__ void filters(const fsc_causal_conv_args& a, int c, int have, float (&w)[K][V], float (&bias)[V]) {
+// Channels c .. c + V - 1 of the U frames from t >= 0 as they lie in memory: U independent loads, which nothing waits for here.  Frames behind the
+// last are read from the last; the caller leaves them out.
+template <typename T, int V, int U>
+__device__ __forceinline__ void fetch(const void* base, long batch, long time, int n, int c, int t, int len, bool wide, int have, fsc::Pack<T, V> (&raw)[U]) {
+    const int last = len - 1 - t;
+    const T* p = reinterpret_cast<const T*>(base) + n * batch + t * time + c;
+    if (wide) {
 #pragma unroll
-    for (int i = 0; i < V; ++i) {
-        bias[i] = i < have && a.bias != nullptr ? a.bias[c + i] : 0.f;
+        for (int j = 0; j < U; ++j) raw[j] = fsc::load_pack<T, V>(p + (j < last ? j : last) * (int)time);
+    } else {
 #pragma unroll
-        for (int k = 0; k < K; ++k) w[k][i] = i < have ? a.weight[(long)(c + i) * K + k] : 0.f;
+        for (int j = 0; j < U; ++j)
+#pragma unroll
+            for (int i = 0; i < V; ++i) raw[j].v[i] = p[(j < last ? j : last) * (int)time + (i < have ? i : have - 1)];
+    }
+}
+template <typename T, int V, int U>
+__device__ __forceinline__ void convert(const fsc::Pack<T, V> (&raw)[U], float (*out)[V]) {
+#pragma unroll
+    for (int j = 0; j < U; ++j)
+#pragma unroll
+        for (int i = 0; i < V; ++i) out[j][i] = (float)raw[j].v[i];
+}
+template <typename T, int V, int U>
+__device__ __forceinline__ void frames(const void* base, long batch, long time, int n, int c, int t, int len, bool wide, int have, float (*out)[V]) {
+    fsc::Pack<T, V> raw[U];
+    fetch<T, V, U>(base, batch, time, n, c, t, len, wide, have, raw);
+    convert<T, V, U>(raw, out);
+}
+
+// The K - 1 frames in front of a strip that begins at t0: frames of x, or (t0 == 0) the given window or zeros.
+template <typename T, int K, int V>
+__device__ __forceinline__ void window(const fsc_causal_conv_args& a, int n, int c, int t0, int len, bool wide, int have, float (*out)[V]) {
+    if constexpr (K > 1) {
+        if (t0 > 0 && t0 - (K - 1) < len) {
+            frames<T, V, K - 1>(a.x, a.x_batch, a.x_time, n, c, t0 - (K - 1), len, wide, have, out);
+        } else if (t0 == 0 && a.initial != nullptr) {
+            frames<T, V, K - 1>(a.initial, (long)(K - 1) * a.channels, a.channels, n, c, 0, K - 1, wide, have, out);
+        } else {
+#pragma unroll
+            for (int j = 0; j < K - 1; ++j)
+#pragma unroll
+                for (int i = 0; i < V; ++i) out[j][i] = 0.f;
+        }
     }
 }
 
+template <int K, int V>
+__device__ __forceinline__ void filters(const fsc_causal_conv_args& a, const Plan& p, int c, int have, float (&w)[K][V], float (&bias)[V]) {
+    static_assert(V == 4, "K quadruples of weights");
+    if (p.wide_weights && have == V) {
+        float flat[V * K];
+        const float* from = a.weight + (long)c * K;
+#pragma unroll
+        for (int q = 0; q < K; ++q) {
+            const fsc::Pack<float, 4> v = fsc::load_pack<float, 4>(from + 4 * q);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) flat[4 * q + i] = v.v[i];
+        }
+#pragma unroll
+        for (int i = 0; i < V; ++i)
+#pragma unroll
+            for (int k = 0; k < K; ++k) w[k][i] = flat[i * K + k];
+    } else {
+#pragma unroll
+        for (int i = 0; i < V; ++i)
+#pragma unroll
+            for (int k = 0; k < K; ++k) w[k][i] = i < have ? a.weight[(long)(c + i) * K + k] : 0.f;
+    }
+#pragma unroll
+    for (int i = 0; i < V; ++i) bias[i] = i < have && a.bias != nullptr ? a.bias[c + i] : 0.f;
+}
+
 template <typename T, int K, int V>
-__global__ __launch_bounds__(kThreads) void conv_fwd_kernel(fsc_causal_conv_args a, Plan p) {
+__global__ __launch_bounds__(kThreads, K <= 4 ? 4 : 3) void conv_fwd_kernel(fsc_causal_conv_args a, Plan p) {
     constexpr int U = 8;
     const int g = blockIdx.y * p.lanes + (threadIdx.x & (p.lanes - 1));
     const long row = (long)blockIdx.x * (kThreads / p.lanes) + threadIdx.x / p.lanes;
@@ -76,29 +141,28 @@ __global__ __launch_bounds__(kThreads) void conv_fwd_kernel(fsc_causal_conv_args
         }
     }
     float w[K][V], bias[V];
-    filters<K, V>(a, c, have, w, bias);
+    filters<K, V>(a, p, c, have, w, bias);
     const int t0 = s * p.strip, t1 = t0 + p.strip < a.length ? t0 + p.strip : a.length;
     float x[K - 1 + U][V];
-#pragma unroll
-    for (int j = 0; j < K - 1; ++j) frame<T, V>(a, n, c, t0 - (K - 1) + j, len, wide, have, x[j]);
+    window<T, K, V>(a, n, c, t0, len, wide, have, x);
     T* out = reinterpret_cast<T*>(a.y) + ((long)n * a.length + t0) * a.channels + c;
     for (int t = t0; t < t1; t += U) {
-#pragma unroll
-        for (int j = 0; j < U; ++j) frame<T, V>(a, n, c, t + j, len, wide, have, x[K - 1 + j]);
+        if (t < len) frames<T, V, U>(a.x, a.x_batch, a.x_time, n, c, t, len, wide, have, x + K - 1);
 #pragma unroll
         for (int j = 0; j < U; ++j) {
-            if (t + j >= t1) break;
             float y[V];
 #pragma unroll
             for (int i = 0; i < V; ++i) {
                 float v = bias[i];
 #pragma unroll
                 for (int k = 0; k < K; ++k) v = fmaf(w[k][i], x[j + k][i], v);
-                y[i] = t + j < len ? (a.silu ? v * sigmoid_fast(v) : v) : 0.f;
+                y[i] = a.silu ? v * sigmoid_fast(v) : v;
+                y[i] = t + j < len ? y[i] : 0.f;
             }
-            store_row<V>(out, wide, have, y);
-            out += a.channels;
+            if (t + j < t1) store_row<V>(out + j * a.channels, wide, have, y);
+            __builtin_amdgcn_sched_barrier(0);       // (else all the frames' sums are in registers at once: two waves fewer a SIMD)
         }
+        out += (long)U * a.channels;
 #pragma unroll
         for (int j = 0; j < K - 1; ++j)
 #pragma unroll
@@ -106,9 +170,10 @@ __global__ __launch_bounds__(kThreads) void conv_fwd_kernel(fsc_causal_conv_args
     }
 }
 
-template <typename T, int K, int V>
+// FINAL: a gradient of the kept frames arrives too (rare: its reads stay out of the other variant's loop).
+template <typename T, int K, int V, bool FINAL>
 __global__ __launch_bounds__(kThreads) void conv_bwd_kernel(fsc_causal_conv_args a, Plan p) {
-    constexpr int U = 4;
+    constexpr int U = K <= 4 ? 8 : 4;
     __shared__ float red[kThreads][V];
     const int lane = threadIdx.x & (p.lanes - 1), sub = threadIdx.x / p.lanes, subs = kThreads / p.lanes;
     const int g = blockIdx.y * p.lanes + lane, c = g * V;
@@ -116,7 +181,7 @@ __global__ __launch_bounds__(kThreads) void conv_bwd_kernel(fsc_causal_conv_args
     const int have = !mine ? 0 : a.channels - c < V ? a.channels - c : V;
     const bool wide = p.wide && mine;
     float w[K][V], bias[V], dw[K][V], db[V];
-    filters<K, V>(a, mine ? c : 0, have, w, bias);
+    filters<K, V>(a, p, mine ? c : 0, have, w, bias);
 #pragma unroll
     for (int i = 0; i < V; ++i) {
         db[i] = 0.f;
@@ -128,66 +193,82 @@ __global__ __launch_bounds__(kThreads) void conv_bwd_kernel(fsc_causal_conv_args
         const int len = frames_of(a, n);
         const int t0 = s * p.strip, t1 = t0 + p.strip < a.length ? t0 + p.strip : a.length;
         float x[K - 1 + U][V], dp[K - 1 + U][V];
+        window<T, K, V>(a, n, c, t0, len, wide, have, x);
 #pragma unroll
-        for (int j = 0; j < K - 1; ++j) {
-            frame<T, V>(a, n, c, t0 - (K - 1) + j, len, wide, have, x[j]);
+        for (int j = 0; j < K - 1; ++j)
 #pragma unroll
             for (int i = 0; i < V; ++i) dp[j][i] = 0.f;
-        }
-        // frame t yields d pre[t]; with it frame t - (K - 1) has its gradient
+        // frame t yields d pre[t]; with it frame t - (K - 1) has its gradient.  The next U frames are on their way while these are worked on:
+        // with two waves a SIMD nothing else covers the loads (4 x 8191 x 2048 in bf16: 142 us without)
+        fsc::Pack<T, V> raw_x[U], raw_dy[U];
+        auto ahead = [&](int t) {
+            if (t < len) {
+                fetch<T, V, U>(a.x, a.x_batch, a.x_time, n, c, t, len, wide, have, raw_x);
+                if (a.dy != nullptr) fetch<T, V, U>(a.dy, a.dy_batch, a.dy_time, n, c, t, len, wide, have, raw_dy);
+            }
+        };
+        ahead(t0);
+        T* out = reinterpret_cast<T*>(a.dx) + ((long)n * a.length + t0 - (K - 1)) * a.channels + c;      // of frame t - (K - 1)
         for (int t = t0; t < t1 + K - 1; t += U) {
             float dy[U][V];
+            convert<T, V, U>(raw_x, x + K - 1);
+            convert<T, V, U>(raw_dy, dy);
+            if (t + U < t1 + K - 1) ahead(t + U);
 #pragma unroll
             for (int j = 0; j < U; ++j) {
-                frame<T, V>(a, n, c, t + j, len, wide, have, x[K - 1 + j]);
-                if (a.dy != nullptr && t + j < len) {
-                    load_row<V>(reinterpret_cast<const T*>(a.dy) + n * a.dy_batch + (t + j) * a.dy_time + c, wide, have, dy[j]);
-                } else {
+                const bool there = t + j < len && a.dy != nullptr, sum = t + j < t1;      // (frames past the strip are summed by the next one)
+                float grad[V];
 #pragma unroll
-                    for (int i = 0; i < V; ++i) dy[j][i] = 0.f;
-                }
-            }
+                for (int i = 0; i < V; ++i) grad[i] = dy[j][i];
+                if (a.silu) {
 #pragma unroll
-            for (int j = 0; j < U; ++j) {
-#pragma unroll
-                for (int i = 0; i < V; ++i) {
-                    float grad = dy[j][i];
-                    if (a.silu) {
+                    for (int i = 0; i < V; ++i) {
                         float v = bias[i];
 #pragma unroll
                         for (int k = 0; k < K; ++k) v = fmaf(w[k][i], x[j + k][i], v);
                         const float sig = sigmoid_fast(v);
-                        grad *= sig * fmaf(v, 1.0f - sig, 1.0f);
+                        grad[i] *= sig * fmaf(v, 1.0f - sig, 1.0f);
                     }
-                    if (t + j >= len) grad = 0.f;
-                    dp[K - 1 + j][i] = grad;
-                    if (t + j < t1) {                              // (the frames past the strip are summed by the next one)
-                        db[i] += grad;
+                }
 #pragma unroll
-                        for (int k = 0; k < K; ++k) dw[k][i] = fmaf(grad, x[j + k][i], dw[k][i]);
+                for (int i = 0; i < V; ++i) {
+                    fsc::pin(grad[i]);               // (computed by every lane: a branch around it would cost more)
+                    grad[i] = there ? grad[i] : 0.f;
+                    dp[K - 1 + j][i] = grad[i];
+                    grad[i] = sum ? grad[i] : 0.f;
+                    db[i] += grad[i];
+                    fsc::pin(db[i]);
+#pragma unroll
+                    for (int k = 0; k < K; ++k) {
+                        dw[k][i] = fmaf(grad[i], x[j + k][i], dw[k][i]);
+                        fsc::pin(dw[k][i]);
                     }
                 }
                 const int at = t + j - (K - 1);
-                if (at >= t1 || (at < t0 && s > 0) || (at < 0 && (a.dinitial == nullptr || at < -(K - 1)))) continue;
                 float dx[V];
 #pragma unroll
                 for (int i = 0; i < V; ++i) {
                     float v = 0.f;
 #pragma unroll
                     for (int k = 0; k < K; ++k) v = fmaf(w[K - 1 - k][i], dp[j + k][i], v);
+                    fsc::pin(v);
                     dx[i] = at < len ? v : 0.f;
                 }
-                const int f = at - len + K - 1;                    // among the kept frames
-                if (a.dfinal != nullptr && f >= 0 && f < K - 1) {
-                    float more[V];
-                    load_row<V>(reinterpret_cast<const T*>(a.dfinal) + ((long)n * (K - 1) + f) * a.channels + c, wide, have, more);
+                if constexpr (FINAL) {
+                    const int f = at - len + K - 1;                    // among the kept frames
+                    if (f >= 0 && f < K - 1 && at < t1 && (at >= t0 || s == 0)) {
+                        float more[V];
+                        load_row<V>(reinterpret_cast<const T*>(a.dfinal) + ((long)n * (K - 1) + f) * a.channels + c, wide, have, more);
 #pragma unroll
-                    for (int i = 0; i < V; ++i) dx[i] += more[i];
+                        for (int i = 0; i < V; ++i) dx[i] += more[i];
+                    }
                 }
-                T* to = at >= 0 ? reinterpret_cast<T*>(a.dx) + ((long)n * a.length + at) * a.channels + c
-                                : reinterpret_cast<T*>(a.dinitial) + ((long)n * (K - 1) + K - 1 + at) * a.channels + c;
-                store_row<V>(to, wide, have, dx);
+                if (at >= t0 && at < t1) store_row<V>(out + j * a.channels, wide, have, dx);
+                else if (at < 0 && at >= 1 - K && a.dinitial != nullptr)
+                    store_row<V>(reinterpret_cast<T*>(a.dinitial) + ((long)n * (K - 1) + K - 1 + at) * a.channels + c, wide, have, dx);
+                __builtin_amdgcn_sched_barrier(0);
             }
+            out += (long)U * a.channels;
 #pragma unroll
             for (int j = 0; j < K - 1; ++j)
 #pragma unroll
@@ -218,29 +299,30 @@ __global__ __launch_bounds__(kThreads) void conv_bwd_kernel(fsc_causal_conv_args
     }
 }
 
-// dweight[c, k] / dbias[c]: the blocks' partial sums, 64 columns x 4 interleaved shares of the blocks
+// dweight[c, k] / dbias[c]: the blocks' partial sums, 32 columns x 8 interleaved shares of the blocks
 __global__ __launch_bounds__(kThreads) void conv_bwd_finish_kernel(const float* __restrict__ part, int parts, int channels, int padded, int taps,
                                                                    float* __restrict__ dweight, float* __restrict__ dbias) {
-    __shared__ float red[4][64];
-    const int column = blockIdx.x * 64 + (threadIdx.x & 63), share = threadIdx.x >> 6;
+    __shared__ float red[8][32];
+    const int lane = threadIdx.x & 31, share = threadIdx.x >> 5, column = blockIdx.x * 32 + lane;
     const long columns = (long)(taps + 1) * padded;
-    float v0 = 0.f, v1 = 0.f;
+    float v[4] = {};
     if (column < columns) {
         int q = share;
-        for (; q + 4 < parts; q += 8) {
-            v0 += part[q * columns + column];
-            v1 += part[(q + 4) * columns + column];
-        }
-        if (q < parts) v0 += part[q * columns + column];
+        for (; q + 24 < parts; q += 32)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) v[i] += part[(q + 8 * i) * columns + column];
+        for (; q < parts; q += 8) v[0] += part[q * columns + column];
     }
-    red[share][threadIdx.x & 63] = v0 + v1;
+    red[share][lane] = (v[0] + v[1]) + (v[2] + v[3]);
     __syncthreads();
     if (share != 0 || column >= columns) return;
+    float sum = 0.f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) sum += red[i][lane];
     const int k = column / padded, c = column % padded;
     if (c >= channels) return;
-    const float v = (red[0][column & 63] + red[1][column & 63]) + (red[2][column & 63] + red[3][column & 63]);
-    if (k < taps) dweight[(long)c * taps + k] = v;
-    else if (dbias != nullptr) dbias[c] = v;
+    if (k < taps) dweight[(long)c * taps + k] = sum;
+    else if (dbias != nullptr) dbias[c] = sum;
 }
 
 // One frame: a thread reads its window, computes, and writes the window one frame on.
@@ -257,7 +339,7 @@ __global__ __launch_bounds__(kThreads) void conv_step_kernel(fsc_causal_conv_arg
 #pragma unroll
     for (int k = 0; k < K - 1; ++k) load_row<V>(window + (long)k * a.channels, wide, have, x[k]);
     load_row<V>(reinterpret_cast<const T*>(a.x) + n * a.x_batch + c, wide, have, x[K - 1]);
-    filters<K, V>(a, c, have, w, bias);
+    filters<K, V>(a, p, c, have, w, bias);
 #pragma unroll
     for (int k = 0; k < K - 1; ++k) store_row<V>(window + (long)k * a.channels, wide, have, x[k + 1]);
 #pragma unroll
@@ -274,12 +356,13 @@ __global__ __launch_bounds__(kThreads) void conv_step_kernel(fsc_causal_conv_arg
 // fill the card.
 constexpr long kWanted = 2 * 1024 * 64;
 
-Plan plan(const fsc_causal_conv_args& a, int v, bool backward) {
+Plan plan(const fsc_causal_conv_args& a) {
+    constexpr int v = kV;
     Plan p{};
     p.groups = fsc::ceil_div(a.channels, v);
     const long frames = (long)a.batch * a.length * p.groups;
     long strip = frames / kWanted / 8 * 8;
-    const long least = backward ? 16 : 8, most = 64;
+    const long least = 8, most = 64;
     strip = strip < least ? least : strip > most ? most : strip;
     p.strip = (int)strip;
     p.strips = a.length > 0 ? fsc::ceil_div(a.length, strip) : 1;
@@ -290,10 +373,9 @@ Plan plan(const fsc_causal_conv_args& a, int v, bool backward) {
     p.wide = a.channels % v == 0 && a.x_batch % v == 0 && a.x_time % v == 0 && a.dy_batch % v == 0 && a.dy_time % v == 0 &&
              fsc::aligned(a.x, unit) && fsc::aligned(a.initial, unit) && fsc::aligned(a.y, unit) && fsc::aligned(a.final, unit) &&
              fsc::aligned(a.dy, unit) && fsc::aligned(a.dfinal, unit) && fsc::aligned(a.dx, unit) && fsc::aligned(a.dinitial, unit);
+    p.wide_weights = fsc::aligned(a.weight, 16);
     return p;
 }
-
-constexpr int kBwdV = 4;
 
 // Blocks along the rows of the backward pass: enough for two blocks a CU, and no more partial sums than that.
 int bwd_parts(const Plan& p) {
@@ -309,6 +391,9 @@ const char* bad(const fsc_causal_conv_args* a) {
     if (a->batch < 0 || a->length < 0 || a->channels < 0) return "negative size";
     if ((long)a->batch * (a->length / 8 + 1) > 0x7FFFFFFFL) return "batch * length is too large";
     if (a->channels > (1 << 23)) return "more than 2^23 channels";
+    const long strides[] = {a->x_time, a->dy_time};
+    for (const long s : strides)
+        if (s < 0 || s > (1L << 26)) return "negative time strides or above 2^26";
     if (a->channels > 0 && a->weight == nullptr) return "null weight";
     return nullptr;
 }
@@ -339,11 +424,10 @@ int fsc_causal_conv_fwd(const fsc_causal_conv_args* args_host, fsc_stream_t stre
     FSC_CHECK_ARG(a.length == 0 || (a.x && a.y), "fsc_causal_conv_fwd: null x or y");
     auto typed = [&](auto type) {
         using T = decltype(type);
-        constexpr int V = 16 / sizeof(T);
-        const Plan p = plan(a, V, false);
+        const Plan p = plan(a);
         const dim3 grid(fsc::ceil_div(p.rows, kThreads / p.lanes), fsc::ceil_div(p.groups, p.lanes));
         with_taps(a.taps, [&](auto taps) {
-            hipLaunchKernelGGL((conv_fwd_kernel<T, decltype(taps)::value, V>), grid, dim3(kThreads), 0, fsc::as_stream(stream), a, p);
+            hipLaunchKernelGGL((conv_fwd_kernel<T, decltype(taps)::value, kV>), grid, dim3(kThreads), 0, fsc::as_stream(stream), a, p);
         });
     };
     FSC_WITH_DTYPE(a.dtype, typed);
@@ -354,8 +438,8 @@ int fsc_causal_conv_fwd(const fsc_causal_conv_args* args_host, fsc_stream_t stre
 size_t fsc_causal_conv_bwd_workspace_bytes(const fsc_causal_conv_args* args_host) {
     if (bad(args_host) != nullptr) return 0;
     const fsc_causal_conv_args& a = *args_host;
-    const Plan p = plan(a, kBwdV, true);
-    return sizeof(float) * (size_t)bwd_parts(p) * (a.taps + 1) * p.groups * kBwdV;
+    const Plan p = plan(a);
+    return sizeof(float) * (size_t)bwd_parts(p) * (a.taps + 1) * p.groups * kV;
 }
 
 int fsc_causal_conv_bwd(const fsc_causal_conv_args* args_host, fsc_stream_t stream) {
@@ -365,19 +449,20 @@ int fsc_causal_conv_bwd(const fsc_causal_conv_args* args_host, fsc_stream_t stre
     if (a.channels == 0) return 0;
     FSC_CHECK_ARG(a.dweight && a.workspace, "fsc_causal_conv_bwd: null dweight or workspace");
     FSC_CHECK_ARG(a.batch == 0 || a.length == 0 || (a.x && a.dx), "fsc_causal_conv_bwd: null x or dx");
-    const Plan p = plan(a, kBwdV, true);
+    const Plan p = plan(a);
     const int parts = bwd_parts(p);
     auto typed = [&](auto type) {
         using T = decltype(type);
         const dim3 grid(parts, fsc::ceil_div(p.groups, p.lanes));
         with_taps(a.taps, [&](auto taps) {
-            hipLaunchKernelGGL((conv_bwd_kernel<T, decltype(taps)::value, kBwdV>), grid, dim3(kThreads), 0, fsc::as_stream(stream), a, p);
+            if (a.dfinal != nullptr) hipLaunchKernelGGL((conv_bwd_kernel<T, decltype(taps)::value, kV, true>), grid, dim3(kThreads), 0, fsc::as_stream(stream), a, p);
+            else hipLaunchKernelGGL((conv_bwd_kernel<T, decltype(taps)::value, kV, false>), grid, dim3(kThreads), 0, fsc::as_stream(stream), a, p);
         });
     };
     FSC_WITH_DTYPE(a.dtype, typed);
     FSC_LAUNCH_CHECK("fsc_causal_conv_bwd");
-    const int padded = p.groups * kBwdV;
-    hipLaunchKernelGGL(conv_bwd_finish_kernel, dim3(fsc::ceil_div((long)(a.taps + 1) * padded, 64)), dim3(kThreads), 0,
+    const int padded = p.groups * kV;
+    hipLaunchKernelGGL(conv_bwd_finish_kernel, dim3(fsc::ceil_div((long)(a.taps + 1) * padded, 32)), dim3(kThreads), 0,
                        fsc::as_stream(stream), reinterpret_cast<const float*>(a.workspace), parts, a.channels, padded, a.taps, a.dweight,
                        a.dbias);
     FSC_LAUNCH_CHECK("fsc_causal_conv_bwd (sums)");
@@ -392,11 +477,10 @@ int fsc_causal_conv_step(const fsc_causal_conv_args* args_host, fsc_stream_t str
     FSC_CHECK_ARG(a.x && a.y && (a.taps == 1 || a.initial), "fsc_causal_conv_step: null x, y or window");
     auto typed = [&](auto type) {
         using T = decltype(type);
-        constexpr int V = 16 / sizeof(T);
-        const Plan p = plan(a, V, false);
+        const Plan p = plan(a);
         const dim3 grid(fsc::ceil_div(a.batch, kThreads / p.lanes), fsc::ceil_div(p.groups, p.lanes));
         with_taps(a.taps, [&](auto taps) {
-            hipLaunchKernelGGL((conv_step_kernel<T, decltype(taps)::value, V>), grid, dim3(kThreads), 0, fsc::as_stream(stream), a, p);
+            hipLaunchKernelGGL((conv_step_kernel<T, decltype(taps)::value, kV>), grid, dim3(kThreads), 0, fsc::as_stream(stream), a, p);
         });
     };
     FSC_WITH_DTYPE(a.dtype, typed);

@@ -23,6 +23,7 @@ __global__ __launch_bounds__(256) void scan_fwd_kernel(fsc_selective_scan_args a
     scan_rates(a, w, rate);
     scan_state(a, w, ENDS ? nullptr : a.initial, h);
     if constexpr (!ENDS) {
+#pragma unroll 4
         for (int q = 0; q < w.segment; ++q) {
             const float ds = end_deltas[w.end_delta(p, q)];
             float e[NS];

@@ -93,7 +93,7 @@ __global__ __launch_bounds__(256) void scan_bwd_ends_kernel(fsc_selective_scan_a
 // The sums of v[0 .. 2 NS) over the channels of a wave (lanes that differ above the L lanes of one channel).  On return v[0 .. kept)
 // hold the sums of the values first .. first + kept - 1.
 template <int L, int NS>
-__device__ __forceinline__ void channel_sums(float (&v)[2 * NS], int lane) {
+__device__ __forceinline__ void channel_sums(float (&v)[2 * NS]) {
     constexpr int N = 2 * NS;
 #pragma unroll
     for (int i = 0; i < N / 2; ++i) {
@@ -116,6 +116,7 @@ __device__ __forceinline__ void channel_sums(float (&v)[2 * NS], int lane) {
     for (int i = 0; i < kept; ++i) {
         if constexpr (L <= 8) v[i] += dpp<0x128>(v[i]);
         if constexpr (L <= 4) v[i] += dpp<0x124>(v[i]);
+        pin(v[i]);
     }
 }
 
@@ -135,6 +136,7 @@ __global__ __launch_bounds__(256, 2) void scan_bwd_kernel(fsc_selective_scan_arg
     float rate[NS], e[NS], da[NS] = {};              // e: exp(delta_{t+1} A) G_{t+1}, what reaches h_t from behind
     scan_rates(a, w, rate);
     scan_state(a, w, a.dfinal, e);
+#pragma unroll 4
     for (int q = p.segments - 1; q > w.segment; --q) {
         const float ds = ws[at.end_deltas + w.end_delta(p, q)];
         float more[NS];
@@ -258,7 +260,11 @@ __global__ __launch_bounds__(256, 2) void scan_bwd_kernel(fsc_selective_scan_arg
                 }
                 gb4[j] = group_sum<L>(gb);
                 ga4[j] = group_sum<L>(ga);
-                channel_sums<L, NS>(v, lane);
+                pin(gb4[j]);
+                pin(ga4[j]);
+#pragma unroll
+                for (int i = 0; i < NS; ++i) pin(da[i]);
+                channel_sums<L, NS>(v);
                 // upper half: dC, lower half: dB; even rows of 16 lanes: the first half of the states, odd rows: the second
                 constexpr int kept = NS >= 2 ? NS / 2 : 1;
                 const int half = lane >> 5, row = (lane >> 4) & 1;

@@ -59,8 +59,12 @@ __device__ __forceinline__ void store_row(T* p, bool wide, int have, const float
 // within 8 (with equal quads: lane ^ 4), 0x140 mirrored within 16 (with equal eights: lane ^ 8), 0x124 / 0x128 turned by 4 / 8 lanes.
 template <int CTRL>
 __device__ __forceinline__ float dpp(float v) {
-    return __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, v), CTRL, 0xf, 0xf, true));
+    return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), CTRL, 0xf, 0xf, true));
 }
+
+// The value is there from here on: sums that nothing reads for a while are otherwise put off, with all their terms kept in registers until
+// then, and lane exchanges end up under a mask, where they cannot be part of the addition.
+__device__ __forceinline__ void pin(float& v) { asm volatile("" : "+v"(v)); }
 
 // The sum over aligned groups of L <= 16 lanes, in every lane of the group.
 template <int L>
