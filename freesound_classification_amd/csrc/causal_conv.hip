@@ -200,9 +200,9 @@ __global__ __launch_bounds__(kThreads) void conv_bwd_kernel(fsc_causal_conv_args
             for (int i = 0; i < V; ++i) dp[j][i] = 0.f;
         // frame t yields d pre[t]; with it frame t - (K - 1) has its gradient.  The next U frames are on their way while these are worked on:
         // with two waves a SIMD nothing else covers the loads (4 x 8191 x 2048 in bf16: 142 us without)
-        fsc::Pack<T, V> raw_x[U], raw_dy[U];
+        fsc::Pack<T, V> raw_x[U] = {}, raw_dy[U] = {};
         auto ahead = [&](int t) {
-            if (t < len) {
+            if (len > 0) {       // (behind the last frame: the last again.  Their gradient is 0, and 0 times what is read must be 0)
                 fetch<T, V, U>(a.x, a.x_batch, a.x_time, n, c, t, len, wide, have, raw_x);
                 if (a.dy != nullptr) fetch<T, V, U>(a.dy, a.dy_batch, a.dy_time, n, c, t, len, wide, have, raw_dy);
             }
