@@ -4,6 +4,8 @@ The optimizers are fused multi-tensor HIP kernels with torch-compatible state di
 """
 import ctypes as C
 import gc
+import itertools
+import operator
 import os
 import warnings
 from functools import partial
@@ -140,6 +142,10 @@ class FusedSGD(Optimizer):
 
 
 _PARAM_DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+# (applied with map: a step looks at every tensor of the model, and the loop in C costs half of one in Python)
+_dtype_of, _grad_of = operator.attrgetter("dtype"), operator.attrgetter("grad")
+_is_cuda = operator.attrgetter("is_cuda")
+_is_contiguous, _address, _numel, _device_number = torch.Tensor.is_contiguous, torch.Tensor.data_ptr, torch.Tensor.numel, torch.Tensor.get_device
 STATE_BLOCK = 256        # elements that share one scale of an 8-bit moment
 
 
@@ -183,41 +189,46 @@ class FusedAdamW(Optimizer):
             with torch.enable_grad():
                 loss = closure()
         _forget_packed_weights()
-        ordinal = 0
+        places = itertools.count()
         for gi, group in enumerate(self.param_groups):
-            batches = {}                         # (dtype, step) -> [(parameter, gradient, state, place)]: one launch sequence each
-            for p in group["params"]:
-                ordinal += 1
-                g = p.grad
-                if g is None or p.numel() == 0:
-                    continue
-                if p.dtype not in _PARAM_DTYPES:
-                    raise _lib.FscError("FusedAdamW: parameters are fp32, bf16 or fp16, got %s" % p.dtype)
-                if g.is_sparse or not p.is_cuda or not g.is_contiguous():
-                    g = _checked_grad(p)
-                if not p.is_contiguous():
-                    raise _lib.FscError("FusedAdamW: parameters must be contiguous")
-                st = self.state[p]
+            params = [(p, place) for p, place in zip(group["params"], places) if p.grad is not None and p.numel() > 0]
+            if not params:
+                continue
+            states = [self.state[p] for p, _ in params]
+            for (p, _), st in zip(params, states):
                 if not st:
                     st.update(self._new_state(p))
-                st["step"] = step = int(st["step"]) + 1
-                batches.setdefault((p.dtype, step), []).append((p, g, st, ordinal - 1))
-            for (dtype, step), entries in batches.items():
-                self._launch(gi, group, dtype, step, entries)
+            ready = [st["step"] for st in states]
+            for st in states:
+                st["step"] = int(st["step"]) + 1
+            # one launch sequence for what shares its type and step count: all of them but for parameters that joined late
+            kinds = list(zip(map(_dtype_of, (p for p, _ in params)), ready))
+            for kind in dict.fromkeys(kinds):
+                if len(set(kinds)) == 1:
+                    chosen, kept = params, states
+                else:
+                    chosen, kept = ([x for x, k in zip(xs, kinds) if k == kind] for xs in (params, states))
+                self._launch(gi, group, kind[0], int(kind[1]) + 1, chosen, kept)
         return loss
 
-    def _launch(self, gi, group, dtype, step, entries):
-        device = entries[0][0].device
-        if any(p.device != device for p, _, _, _ in entries) or device.index != _lib._get_device():
+    def _launch(self, gi, group, dtype, step, params, states):
+        if dtype not in _PARAM_DTYPES:
+            raise _lib.FscError("FusedAdamW: parameters are fp32, bf16 or fp16, got %s" % dtype)
+        tensors = [p for p, _ in params]
+        grads = list(map(_grad_of, tensors))
+        if not all(map(_is_cuda, tensors)) or not all(map(_is_contiguous, grads)):
+            grads = [_checked_grad(p) for p in tensors]
+        if set(map(_device_number, tensors)) != {_lib._get_device()}:
             raise _lib.FscError("FusedAdamW: the parameters of a group must be on the current device")
-        n = len(entries)
-        table = np.zeros((n, 8), dtype=np.int64)
-        table[:, 0] = [e[0].data_ptr() for e in entries]
-        table[:, 1] = [e[1].data_ptr() for e in entries]
-        for column, key in enumerate(self._keys()):
-            table[:, 2 + column] = [e[2][key].data_ptr() for e in entries]
-        table[:, 6] = [e[0].numel() for e in entries]
-        table[:, 7] = [(self.seed + e[3]) & 0xFFFFFFFF for e in entries]
+        if not all(map(_is_contiguous, tensors)):
+            raise _lib.FscError("FusedAdamW: parameters must be contiguous")
+        n = len(tensors)
+        table = np.zeros((8, n), dtype=np.int64)
+        for row, values in enumerate([tensors, grads] + [map(operator.itemgetter(key), states) for key in self._keys()]):
+            table[row] = np.fromiter(map(_address, values), np.int64, n)
+        counts = table[6] = np.fromiter(map(_numel, tensors), np.int64, n)
+        table[7] = (np.fromiter((place for _, place in params), np.int64, n) + (self.seed & 0xFFFFFFFF)) & 0xFFFFFFFF
+        table = np.ascontiguousarray(table.T)
         b1, b2 = group["betas"]
         factors, dev = None, None
         if self.factors_dev is not None:
@@ -226,9 +237,8 @@ class FusedAdamW(Optimizer):
             factors = (C.c_float * 4)()
             _lib.load().fsc_adamw_step_factors(float(group["lr"]), b1, b2, float(group["weight_decay"]), step, factors)
         from .. import functional as F
-        count = int(table[:, 6].sum())
         held = 8 if self.state_bits == 32 else 2
-        with F._stage("optimizer", count * (3 * entries[0][0].element_size() + 2 * held)):
+        with F._stage("optimizer", int(counts.sum()) * (3 * tensors[0].element_size() + 2 * held)):
             call("fsc_adamw_step", table.ctypes.data, n, _PARAM_DTYPES[dtype], self.state_bits, factors, dev, b1, b2,
                  float(group["eps"]), float(self.grad_scale), stream_ptr())
 
