@@ -91,19 +91,6 @@ __device__ __forceinline__ void swap16(float& a, float& b) {
     b = __builtin_bit_cast(float, second);
 }
 
-// The largest value of the wave, in every lane; no value is NaN.
-__device__ __forceinline__ float wave_top(float v) {
-    v = fmaxf(v, dpp<0xB1>(v));
-    v = fmaxf(v, dpp<0x4E>(v));
-    v = fmaxf(v, dpp<0x141>(v));
-    v = fmaxf(v, dpp<0x140>(v));
-    float w = v;
-    swap16(v, w);
-    v = w = fmaxf(v, w);
-    swap32(v, w);
-    return fmaxf(v, w);
-}
-
 inline size_t dtype_bytes(int dtype) { return dtype == FSC_DTYPE_F32 ? 4 : 2; }
 inline bool dtype_ok(int dtype) { return dtype == FSC_DTYPE_F32 || dtype == FSC_DTYPE_BF16 || dtype == FSC_DTYPE_F16; }
 // whether `bytes`-wide accesses at p + multiples of `strides` elements stay aligned

@@ -4,7 +4,6 @@ The optimizers are fused multi-tensor HIP kernels with torch-compatible state di
 """
 import ctypes as C
 import gc
-import itertools
 import operator
 import os
 import warnings
@@ -143,7 +142,8 @@ class FusedSGD(Optimizer):
 
 _PARAM_DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 # (applied with map: a step looks at every tensor of the model, and the loop in C costs half of one in Python)
-_dtype_of, _grad_of = operator.attrgetter("dtype"), operator.attrgetter("grad")
+_dtype_of, _grad_of, _step_of = operator.attrgetter("dtype"), operator.attrgetter("grad"), operator.itemgetter("step")
+_is_none = partial(operator.is_, None)
 _is_cuda = operator.attrgetter("is_cuda")
 _is_contiguous, _address, _numel, _device_number = torch.Tensor.is_contiguous, torch.Tensor.data_ptr, torch.Tensor.numel, torch.Tensor.get_device
 STATE_BLOCK = 256        # elements that share one scale of an 8-bit moment
@@ -189,32 +189,35 @@ class FusedAdamW(Optimizer):
             with torch.enable_grad():
                 loss = closure()
         _forget_packed_weights()
-        places = itertools.count()
+        place = 0
         for gi, group in enumerate(self.param_groups):
-            params = [(p, place) for p, place in zip(group["params"], places) if p.grad is not None and p.numel() > 0]
+            params, salts = group["params"], np.arange(place, place + len(group["params"]))
+            place += len(params)
+            missing = list(map(_is_none, map(_grad_of, params)))
+            if any(missing):
+                params, salts = [p for p, none in zip(params, missing) if not none], salts[np.logical_not(missing)]
             if not params:
                 continue
-            states = [self.state[p] for p, _ in params]
-            for (p, _), st in zip(params, states):
-                if not st:
-                    st.update(self._new_state(p))
-            ready = [st["step"] for st in states]
+            states = [self.state[p] for p in params]
+            if not all(states):
+                for p, st in zip(params, states):
+                    if not st:
+                        st.update(self._new_state(p))
+            # one launch sequence for what shares its type and step count: all of them but for parameters that joined late
+            kinds = list(zip(map(_dtype_of, params), map(_step_of, states)))
             for st in states:
                 st["step"] = int(st["step"]) + 1
-            # one launch sequence for what shares its type and step count: all of them but for parameters that joined late
-            kinds = list(zip(map(_dtype_of, (p for p, _ in params)), ready))
             for kind in dict.fromkeys(kinds):
-                if len(set(kinds)) == 1:
-                    chosen, kept = params, states
-                else:
-                    chosen, kept = ([x for x, k in zip(xs, kinds) if k == kind] for xs in (params, states))
-                self._launch(gi, group, kind[0], int(kind[1]) + 1, chosen, kept)
+                chosen = params, states, salts
+                if kinds.count(kind) != len(kinds):
+                    at = [i for i, k in enumerate(kinds) if k == kind]
+                    chosen = [params[i] for i in at], [states[i] for i in at], salts[at]
+                self._launch(gi, group, kind[0], int(kind[1]) + 1, *chosen)
         return loss
 
-    def _launch(self, gi, group, dtype, step, params, states):
+    def _launch(self, gi, group, dtype, step, tensors, states, salts):
         if dtype not in _PARAM_DTYPES:
             raise _lib.FscError("FusedAdamW: parameters are fp32, bf16 or fp16, got %s" % dtype)
-        tensors = [p for p, _ in params]
         grads = list(map(_grad_of, tensors))
         if not all(map(_is_cuda, tensors)) or not all(map(_is_contiguous, grads)):
             grads = [_checked_grad(p) for p in tensors]
@@ -227,7 +230,7 @@ class FusedAdamW(Optimizer):
         for row, values in enumerate([tensors, grads] + [map(operator.itemgetter(key), states) for key in self._keys()]):
             table[row] = np.fromiter(map(_address, values), np.int64, n)
         counts = table[6] = np.fromiter(map(_numel, tensors), np.int64, n)
-        table[7] = (np.fromiter((place for _, place in params), np.int64, n) + (self.seed & 0xFFFFFFFF)) & 0xFFFFFFFF
+        table[7] = (salts + (self.seed & 0xFFFFFFFF)) & 0xFFFFFFFF
         table = np.ascontiguousarray(table.T)
         b1, b2 = group["betas"]
         factors, dev = None, None
