@@ -50,7 +50,7 @@ __device__ __forceinline__ void frame(const fsc_causal_conv_args& a, int n, int 
     }
 }
 
-// Channels c .. c + V - 1 of the U frames from t >= 0 as they lie in memory: U independent loads, which nothing waits for here.  Frames behind the
+// Channels c .. c + V - 1 of the U frames from t, 0 <= t < len, as they lie in memory: U independent loads, which nothing waits for here.  Frames behind the
 // last are read from the last; the caller leaves them out.
 template <typename T, int V, int U>
 __device__ __forceinline__ void fetch(const void* base, long batch, long time, int n, int c, int t, int len, bool wide, int have, fsc::Pack<T, V> (&raw)[U]) {
@@ -202,7 +202,7 @@ __global__ __launch_bounds__(kThreads) void conv_bwd_kernel(fsc_causal_conv_args
         // with two waves a SIMD nothing else covers the loads (4 x 8191 x 2048 in bf16: 142 us without)
         fsc::Pack<T, V> raw_x[U] = {}, raw_dy[U] = {};
         auto ahead = [&](int t) {
-            if (len > 0) {       // (behind the last frame: the last again.  Their gradient is 0, and 0 times what is read must be 0)
+            if (t < len) {       // (behind the end the last values stay, or the zeros: their gradient is 0 and must meet a number)
                 fetch<T, V, U>(a.x, a.x_batch, a.x_time, n, c, t, len, wide, have, raw_x);
                 if (a.dy != nullptr) fetch<T, V, U>(a.dy, a.dy_batch, a.dy_time, n, c, t, len, wide, have, raw_dy);
             }

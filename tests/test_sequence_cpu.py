@@ -31,7 +31,8 @@ def test_conv_entry_points_refuse_bad_arguments(name):
     _refused(name, None, None, match="null arguments")
     for kw, text in ((dict(taps=0), "taps"), (dict(taps=9), "taps"), (dict(dtype=3), "dtype"), (dict(batch=-1), "negative"),
                      (dict(), "null weight"), (dict(channels=(1 << 23) + 1, weight=64), "channels"),
-                     (dict(batch=2 ** 30, length=2 ** 30, weight=64), "too large"), (dict(weight=64), "null")):
+                     (dict(batch=2 ** 30, length=2 ** 30, weight=64), "too large"), (dict(weight=64), "null"),
+                     (dict(weight=64, x_time=2 ** 26 + 1), "strides"), (dict(weight=64, dy_time=-1), "strides")):
         _refused(name, C.byref(_conv(**kw)), None, match=text)
 
 
@@ -40,7 +41,7 @@ def test_scan_entry_points_refuse_bad_arguments(name):
     _refused(name, None, None, match="null arguments")
     for kw, text in ((dict(states=0), "states"), (dict(states=65), "states"), (dict(groups=3), "groups"), (dict(groups=0), "groups"),
                      (dict(dtype=-1), "dtype"), (dict(length=-1), "negative"), (dict(a_log=None), "a_log"),
-                     (dict(batch=2 ** 30), "too large"), (dict(), "null")):
+                     (dict(batch=2 ** 30), "too large"), (dict(), "null"), (dict(b_time=2 ** 26 + 1), "strides"), (dict(dy_time=-1), "strides")):
         _refused(name, C.byref(_scan(**kw)), None, match=text)
 
 

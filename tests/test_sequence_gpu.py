@@ -292,6 +292,39 @@ def test_offsets_beyond_32_bits():
     torch.cuda.empty_cache()
 
 
+def test_short_sequences_in_long_padding():
+    """One frame of 70 000 that exist, 2^15 elements apart: no offset from behind the end is formed in 32 bits."""
+    t, d, far = 70000, 8, 2 ** 15
+    base = torch.zeros(t * far + d, dtype=torch.bfloat16, device=DEV)
+    x = base.as_strided((1, t, d), (0, far, 1))
+    gen = torch.Generator(device=DEV).manual_seed(5)
+    small = torch.randn(1, 1, d, generator=gen, device=DEV).bfloat16()
+    x[:, :1] = small
+    w, one = torch.rand(d, 4, generator=gen, device=DEV), torch.ones(1, dtype=torch.int32, device=DEV)
+    results = []
+    for v, lengths in ((x, one), (small, None)):
+        leaf, wl = v.detach().requires_grad_(), w.clone().requires_grad_()
+        y = F.causal_conv(leaf, wl, lengths=lengths)
+        z = F.selective_scan(leaf, leaf, w, leaf[..., :4], leaf[..., 4:], lengths=lengths)
+        g = torch.ones_like(small).expand(1, v.shape[1], d)
+        results.append([y, z] + list(torch.autograd.grad([y, z], [leaf, wl], [g, g])))
+    for a, b in zip(*results):
+        assert torch.equal(a[:, :1] if a.dim() == 3 else a, b) and (a.dim() < 3 or not a[:, 1:].any())
+    del base, x, results
+    torch.cuda.empty_cache()
+
+
+def test_frames_far_apart_are_copied():
+    """A time stride above 2^26 elements, which the kernels refuse."""
+    d, far = 4, 2 ** 26 + 4
+    base = torch.zeros(2 * far, dtype=torch.bfloat16, device=DEV)
+    x = base.as_strided((1, 2, d), (0, far, 1))
+    x.copy_(torch.arange(2 * d, device=DEV).view(1, 2, d))
+    w, rows = torch.ones(d, 2, device=DEV), torch.ones(1, 2, 3, device=DEV, dtype=torch.bfloat16)
+    assert torch.equal(F.causal_conv(x, w), F.causal_conv(x.contiguous(), w))
+    assert torch.equal(F.selective_scan(x, x, w.new_zeros(d, 3), rows, rows), F.selective_scan(x.contiguous(), x.contiguous(), w.new_zeros(d, 3), rows, rows))
+
+
 def test_equal_inputs_give_equal_bits():
     p, lengths, cot = scan_inputs(6, 150, 200, 16, 2, "dzbil", torch.bfloat16, 9)
     dl = torch.tensor(lengths, dtype=torch.int32, device=DEV)
