@@ -144,7 +144,6 @@ _PARAM_DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 # (applied with map: a step looks at every tensor of the model, and the loop in C costs half of one in Python)
 _dtype_of, _grad_of, _step_of = operator.attrgetter("dtype"), operator.attrgetter("grad"), operator.itemgetter("step")
 _is_none = partial(operator.is_, None)
-_is_cuda = operator.attrgetter("is_cuda")
 _is_contiguous, _address, _numel, _device_number = torch.Tensor.is_contiguous, torch.Tensor.data_ptr, torch.Tensor.numel, torch.Tensor.get_device
 STATE_BLOCK = 256        # elements that share one scale of an 8-bit moment
 
@@ -219,9 +218,10 @@ class FusedAdamW(Optimizer):
         if dtype not in _PARAM_DTYPES:
             raise _lib.FscError("FusedAdamW: parameters are fp32, bf16 or fp16, got %s" % dtype)
         grads = list(map(_grad_of, tensors))
-        if not all(map(_is_cuda, tensors)) or not all(map(_is_contiguous, grads)):
+        here = set(map(_device_number, tensors)) == {_lib._get_device()}
+        if not here or not all(map(_is_contiguous, grads)):
             grads = [_checked_grad(p) for p in tensors]
-        if set(map(_device_number, tensors)) != {_lib._get_device()}:
+        if not here:
             raise _lib.FscError("FusedAdamW: the parameters of a group must be on the current device")
         if not all(map(_is_contiguous, tensors)):
             raise _lib.FscError("FusedAdamW: parameters must be contiguous")
