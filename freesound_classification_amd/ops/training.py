@@ -142,7 +142,8 @@ class FusedSGD(Optimizer):
 
 _PARAM_DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 # (applied with map: a step looks at every tensor of the model, and the loop in C costs half of one in Python)
-_dtype_of, _grad_of, _step_of = operator.attrgetter("dtype"), operator.attrgetter("grad"), operator.itemgetter("step")
+_dtype_of, _grad_of = operator.attrgetter("dtype"), operator.attrgetter("grad")
+_step_of, _average_of = operator.itemgetter("step"), operator.itemgetter("exp_avg")
 _is_none = partial(operator.is_, None)
 _is_contiguous, _address, _numel, _device_number = torch.Tensor.is_contiguous, torch.Tensor.data_ptr, torch.Tensor.numel, torch.Tensor.get_device
 STATE_BLOCK = 256        # elements that share one scale of an 8-bit moment
@@ -155,7 +156,8 @@ class FusedAdamW(Optimizer):
     with one fp32 scale per 256 elements -- exp_avg / exp_avg_scale, and the square root of the second moment, exp_avg_sq_root /
     exp_avg_sq_root_scale --, 2.03 bytes a parameter instead of 8, rounded stochastically: the random bits are a function of (`seed`, the
     tensor's place in the optimizer, the step, the element), so a run is reproducible.  Parameters and gradients are fp32, bf16 or fp16.
-    `grad_scale` multiplies gradients first (1 / world_size after a summing all-reduce)."""
+    `grad_scale` multiplies gradients first (1 / world_size after a summing all-reduce).  A refused step changes nothing in its group; a
+    step is recorded into a HIP graph by CapturedTrainingStep alone (elsewhere the step count would be frozen into it)."""
 
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, state_bits=32, seed=0):
         if state_bits not in (32, 8):
@@ -181,56 +183,81 @@ class FusedAdamW(Optimizer):
                 st[key] = torch.zeros(p.shape, device=p.device, dtype=torch.float32 if self.state_bits == 32 else torch.float8_e4m3fn)
         return st
 
+    def add_param_group(self, param_group):
+        super().add_param_group(param_group)
+        params = self.param_groups[-1]["params"]
+        if len(set(map(id, params))) != len(params):         # (one launch updates them side by side: twice would be a race)
+            self.param_groups.pop()
+            raise ValueError("FusedAdamW: a parameter appears more than once in a group")
+
     @torch.no_grad()
     def step(self, closure=None):
         loss = None
         if closure is not None:
             with torch.enable_grad():
                 loss = closure()
+        if self.factors_dev is None and torch.cuda.is_available() and torch.cuda.is_current_stream_capturing():
+            raise _lib.FscError("FusedAdamW: a recorded step would repeat this step's bias corrections; record it with CapturedTrainingStep")
         _forget_packed_weights()
         place = 0
         for gi, group in enumerate(self.param_groups):
             params, salts = group["params"], np.arange(place, place + len(group["params"]))
             place += len(params)
-            missing = list(map(_is_none, map(_grad_of, params)))
+            grads = list(map(_grad_of, params))
+            missing = list(map(_is_none, grads))
             if any(missing):
                 params, salts = [p for p, none in zip(params, missing) if not none], salts[np.logical_not(missing)]
+                grads = list(map(_grad_of, params))
             if not params:
                 continue
-            states = [self.state[p] for p in params]
+            types, counts = list(map(_dtype_of, params)), list(map(_numel, params))
+            grads = self._checked(params, grads, types, counts)
+            states = list(map(self.state.__getitem__, params))
             if not all(states):
                 for p, st in zip(params, states):
                     if not st:
                         st.update(self._new_state(p))
+            averages = list(map(_average_of, states))
+            if set(map(_device_number, averages)) != {_lib._get_device()} or list(map(_numel, averages)) != counts:
+                raise _lib.FscError("FusedAdamW: the moments are not on the parameters' device or not of their size")
+            steps = list(map(_step_of, states))
+            chosen = params, grads, averages, states, salts, counts
+            kind, *others = dict.fromkeys(zip(types, steps)) if len(set(types)) > 1 or len(set(steps)) > 1 else [(types[0], steps[0])]
+            if not others:
+                self._launch(gi, group, *kind, *chosen)
+                continue
             # one launch sequence for what shares its type and step count: all of them but for parameters that joined late
-            kinds = list(zip(map(_dtype_of, params), map(_step_of, states)))
-            for st in states:
-                st["step"] = int(st["step"]) + 1
-            for kind in dict.fromkeys(kinds):
-                chosen = params, states, salts
-                if kinds.count(kind) != len(kinds):
-                    at = [i for i, k in enumerate(kinds) if k == kind]
-                    chosen = [params[i] for i in at], [states[i] for i in at], salts[at]
-                self._launch(gi, group, kind[0], int(kind[1]) + 1, *chosen)
+            for kind in (kind, *others):
+                at = [i for i, k in enumerate(zip(types, steps)) if k == kind]
+                self._launch(gi, group, *kind, *[[values[i] for i in at] for values in chosen])
         return loss
 
-    def _launch(self, gi, group, dtype, step, tensors, states, salts):
-        if dtype not in _PARAM_DTYPES:
-            raise _lib.FscError("FusedAdamW: parameters are fp32, bf16 or fp16, got %s" % dtype)
-        grads = list(map(_grad_of, tensors))
-        here = set(map(_device_number, tensors)) == {_lib._get_device()}
-        if not here or not all(map(_is_contiguous, grads)):
-            grads = [_checked_grad(p) for p in tensors]
-        if not here:
+    @staticmethod
+    def _checked(params, grads, types, counts):
+        """The gradients, contiguous; nothing has changed yet when this refuses."""
+        devices = set(map(_device_number, params + grads))
+        if -1 in devices:
+            raise _lib.FscError("FusedAdamW needs device parameters (no CPU fallback)")
+        if devices != {_lib._get_device()}:
             raise _lib.FscError("FusedAdamW: the parameters of a group must be on the current device")
-        if not all(map(_is_contiguous, tensors)):
+        if not _PARAM_DTYPES.keys() >= set(types):
+            raise _lib.FscError("FusedAdamW: parameters are fp32, bf16 or fp16, got %s" % sorted(map(str, set(types) - _PARAM_DTYPES.keys())))
+        if not all(map(_is_contiguous, params)):
             raise _lib.FscError("FusedAdamW: parameters must be contiguous")
+        if not all(map(_is_contiguous, grads)):
+            grads = [_checked_grad(p) for p in params]
+        if list(map(_dtype_of, grads)) != types or list(map(_numel, grads)) != counts:
+            raise _lib.FscError("FusedAdamW: a gradient's type or size is not its parameter's")
+        return grads
+
+    def _launch(self, gi, group, dtype, step, tensors, grads, averages, states, salts, counts):
+        step = int(step) + 1
         n = len(tensors)
         table = np.zeros((8, n), dtype=np.int64)
-        for row, values in enumerate([tensors, grads] + [map(operator.itemgetter(key), states) for key in self._keys()]):
+        for row, values in enumerate([tensors, grads, averages] + [map(operator.itemgetter(key), states) for key in self._keys()[1:]]):
             table[row] = np.fromiter(map(_address, values), np.int64, n)
-        counts = table[6] = np.fromiter(map(_numel, tensors), np.int64, n)
-        table[7] = (salts + (self.seed & 0xFFFFFFFF)) & 0xFFFFFFFF
+        table[6] = counts
+        table[7] = (np.asarray(salts) + (self.seed & 0xFFFFFFFF)) & 0xFFFFFFFF
         table = np.ascontiguousarray(table.T)
         b1, b2 = group["betas"]
         factors, dev = None, None
@@ -241,9 +268,11 @@ class FusedAdamW(Optimizer):
             _lib.load().fsc_adamw_step_factors(float(group["lr"]), b1, b2, float(group["weight_decay"]), step, factors)
         from .. import functional as F
         held = 8 if self.state_bits == 32 else 2
-        with F._stage("optimizer", int(counts.sum()) * (3 * tensors[0].element_size() + 2 * held)):
+        with F._stage("optimizer", sum(counts) * (3 * tensors[0].element_size() + 2 * held)):
             call("fsc_adamw_step", table.ctypes.data, n, _PARAM_DTYPES[dtype], self.state_bits, factors, dev, b1, b2,
                  float(group["eps"]), float(self.grad_scale), stream_ptr())
+        for st in states:
+            st["step"] = step
 
     def state_dict(self):
         out = super().state_dict()

@@ -270,3 +270,47 @@ def test_refusals():
     r.grad = torch.zeros(8, 3, device=DEV).to_sparse()
     with pytest.raises(RuntimeError):
         FusedAdamW([r]).step()
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_refusals_after_a_step(bits):
+    """Moments of another size or device than the parameter's, a gradient of another type, a plain recording: refused, and nothing changes."""
+    p = torch.nn.Parameter(torch.ones(600, device=DEV))
+    p.grad = torch.ones_like(p)
+    opt = FusedAdamW([p], state_bits=bits)
+    opt.step()
+    held = {key: value for key, value in opt.state[p].items()}
+    before = p.detach().clone()
+
+    def refused():
+        with pytest.raises(FscError):
+            opt.step()
+        assert torch.equal(p.detach(), before) and opt.state[p]["step"] == 1
+
+    opt.state[p]["exp_avg"] = held["exp_avg"].cpu()
+    refused()
+    opt.state[p]["exp_avg"] = held["exp_avg"][:599]
+    refused()
+    opt.state[p]["exp_avg"] = held["exp_avg"]
+    grad = p.grad
+    p.grad = None
+    p.grad_dtype = torch.bfloat16
+    p.grad = torch.ones(600, device=DEV, dtype=torch.bfloat16)
+    refused()
+    p.grad = None
+    p.grad_dtype = torch.float32
+    p.grad = grad
+    stream = torch.cuda.Stream()
+    with torch.cuda.stream(stream):
+        graph, other = torch.cuda.CUDAGraph(), torch.zeros(8, device=DEV)
+        with torch.cuda.graph(graph, stream=stream):
+            other.add_(1.0)
+            refused_here = False
+            try:
+                opt.step()
+            except FscError:
+                refused_here = True
+    torch.cuda.synchronize()
+    assert refused_here and torch.equal(p.detach(), before) and opt.state[p]["step"] == 1
+    opt.step()
+    assert opt.state[p]["step"] == 2 and not torch.equal(p.detach(), before)

@@ -1,5 +1,6 @@
 """Sequence operators and AdamW without a device: argument checks of the Python layer and of the C ABI, plan arithmetic, the 8-bit format."""
 import ctypes as C
+import warnings
 
 import numpy as np
 import pytest
@@ -129,6 +130,19 @@ def test_optimizer_registry_and_groups():
     m[0].weight.grad = torch.zeros_like(m[0].weight)
     with pytest.raises(_lib.FscError, match="device parameters"):
         opt.step()
+
+
+def test_refused_steps_leave_nothing_behind():
+    p, q = (torch.nn.Parameter(torch.zeros(4)) for _ in range(2))
+    with warnings.catch_warnings():
+        warnings.simplefilter("ignore")
+        with pytest.raises(ValueError, match="more than once"):
+            training.FusedAdamW([p, q, p])
+    opt = training.FusedAdamW([p])
+    p.grad = torch.zeros(4)
+    with pytest.raises(_lib.FscError):
+        opt.step()
+    assert not opt.state[p]                      # (moments made on the host would be read by a kernel once the parameter is on the device)
 
 
 def test_held_values():
