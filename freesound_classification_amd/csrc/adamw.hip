@@ -18,6 +18,7 @@ namespace {
 constexpr int kBatch = 52;       // tensors per launch: 52 x 64 bytes of the 4 KB of kernel arguments
 constexpr int kChunk = 4096;     // elements per workgroup: 16 blocks of 256, four per wave
 constexpr int kThreads = 256;
+constexpr long kMostChunks = (1L << 24) - 1;       // of one launch: fewer than 2^32 threads
 constexpr int kBlock = 256;
 constexpr float kTop = 448.0f;   // the largest e4m3 value
 
@@ -302,7 +303,7 @@ int fsc_adamw_step(const fsc_adamw_tensor* tensors_host, int n_tensors, int dtyp
         FSC_CHECK_ARG(t.count >= 0, "fsc_adamw_step: tensor %d has %ld elements", i, t.count);
         FSC_CHECK_ARG(t.count == 0 || (t.param && t.grad && t.state0 && t.state1), "fsc_adamw_step: tensor %d has null pointers", i);
         FSC_CHECK_ARG(t.count == 0 || state_bits == 32 || (t.scale0 && t.scale1), "fsc_adamw_step: tensor %d misses its scales", i);
-        FSC_CHECK_ARG(t.count <= (long)kChunk * 0x3FFFFFFF, "fsc_adamw_step: tensor %d is too large", i);
+        FSC_CHECK_ARG(t.count <= kChunk * kMostChunks, "fsc_adamw_step: tensor %d is too large", i);
     }
     Hyper h{};
     if (factors4 != nullptr) {
@@ -326,7 +327,7 @@ int fsc_adamw_step(const fsc_adamw_tensor* tensors_host, int n_tensors, int dtyp
         while (next < n_tensors && tb.n < kBatch) {
             const fsc_adamw_tensor& t = tensors_host[next];
             const long more = (t.count + kChunk - 1) / kChunk;
-            if (tb.n > 0 && chunks + more > 0x3FFFFFFF) break;
+            if (tb.n > 0 && chunks + more > kMostChunks) break;
             ++next;
             if (more == 0) continue;
             tb.t[tb.n] = t;

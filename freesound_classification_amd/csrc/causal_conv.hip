@@ -355,6 +355,7 @@ __global__ __launch_bounds__(kThreads) void conv_step_kernel(fsc_causal_conv_arg
 // Threads wanted in flight: two waves on each of the 1024 SIMDs.  Long strips read fewer frames twice (K - 1 at each end), short ones
 // fill the card.
 constexpr long kWanted = 2 * 1024 * 64;
+constexpr long kMostBlocks = 1L << 24;       // of one launch: 2^32 threads and more are refused
 
 Plan plan(const fsc_causal_conv_args& a) {
     constexpr int v = kV;
@@ -422,10 +423,11 @@ int fsc_causal_conv_fwd(const fsc_causal_conv_args* args_host, fsc_stream_t stre
     const fsc_causal_conv_args& a = *args_host;
     if (a.batch == 0 || a.channels == 0 || (a.length == 0 && a.final == nullptr)) return 0;
     FSC_CHECK_ARG(a.length == 0 || (a.x && a.y), "fsc_causal_conv_fwd: null x or y");
+    const Plan p = plan(a);
+    const dim3 grid(fsc::ceil_div(p.rows, kThreads / p.lanes), fsc::ceil_div(p.groups, p.lanes));
+    FSC_CHECK_ARG((long)grid.x * grid.y < kMostBlocks, "fsc_causal_conv_fwd: batch * length * channels is too large");
     auto typed = [&](auto type) {
         using T = decltype(type);
-        const Plan p = plan(a);
-        const dim3 grid(fsc::ceil_div(p.rows, kThreads / p.lanes), fsc::ceil_div(p.groups, p.lanes));
         with_taps(a.taps, [&](auto taps) {
             hipLaunchKernelGGL((conv_fwd_kernel<T, decltype(taps)::value, kV>), grid, dim3(kThreads), 0, fsc::as_stream(stream), a, p);
         });
@@ -475,10 +477,11 @@ int fsc_causal_conv_step(const fsc_causal_conv_args* args_host, fsc_stream_t str
     const fsc_causal_conv_args& a = *args_host;
     if (a.batch == 0 || a.channels == 0) return 0;
     FSC_CHECK_ARG(a.x && a.y && (a.taps == 1 || a.initial), "fsc_causal_conv_step: null x, y or window");
+    const Plan p = plan(a);
+    const dim3 grid(fsc::ceil_div(a.batch, kThreads / p.lanes), fsc::ceil_div(p.groups, p.lanes));
+    FSC_CHECK_ARG((long)grid.x * grid.y < kMostBlocks, "fsc_causal_conv_step: batch * channels is too large");
     auto typed = [&](auto type) {
         using T = decltype(type);
-        const Plan p = plan(a);
-        const dim3 grid(fsc::ceil_div(a.batch, kThreads / p.lanes), fsc::ceil_div(p.groups, p.lanes));
         with_taps(a.taps, [&](auto taps) {
             hipLaunchKernelGGL((conv_step_kernel<T, decltype(taps)::value, kV>), grid, dim3(kThreads), 0, fsc::as_stream(stream), a, p);
         });

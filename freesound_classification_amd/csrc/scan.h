@@ -10,6 +10,8 @@
 // Where sequences x channel blocks do not fill the card, time is cut into segments: a first launch computes each segment's end from zero
 // (and the sum of its delta: exp(A sum) is the segment's decay), the main launch joins the ends in front of its own segment.
 #pragma once
+#include <float.h>
+
 #include "seq.h"
 
 namespace fsc {
@@ -60,6 +62,9 @@ inline ScanPlan scan_plan(const fsc_selective_scan_args& a) {
              fits(a.ddt, 0, 0) && fits(a.dz, 0, 0);
     return p;
 }
+
+// Workgroups of 256 threads that one launch takes: fewer than 2^32 threads.
+constexpr long kMostBlocks = (1L << 24) - 1;
 
 inline const char* scan_bad(const fsc_selective_scan_args* a) {
     if (a == nullptr) return "null arguments";
@@ -243,13 +248,19 @@ __device__ __forceinline__ T* scan_out(const fsc_selective_scan_args& a, const S
     return reinterpret_cast<T*>(at + ((uint32_t)w.te * (uint32_t)a.channels + w.ce) * (uint32_t)sizeof(T));
 }
 
-// A = -exp(a_log) of the lane's states, 0 for states that do not exist.
+// A = -exp(a_log), kept finite (a state that forgets everything passes frames with delta = 0 unchanged all the same); NaN stays NaN.
+__device__ __forceinline__ float rate_of(float a_log) {
+    const float e = expf(a_log);
+    return e > FLT_MAX ? -FLT_MAX : -e;
+}
+
+// A of the lane's states, 0 for states that do not exist.
 template <int L, int NS>
 __device__ __forceinline__ void scan_rates(const fsc_selective_scan_args& a, const ScanPlace<L, NS>& w, float (&rate)[NS]) {
 #pragma unroll
     for (int i = 0; i < NS; ++i) {
         const int s = w.sg * NS + i;
-        rate[i] = w.real && s < a.states ? -expf(a.a_log[(long)w.channel * a.states + s]) : 0.f;
+        rate[i] = w.real && s < a.states ? rate_of(a.a_log[(long)w.channel * a.states + s]) : 0.f;
     }
 }
 

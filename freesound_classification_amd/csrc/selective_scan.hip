@@ -165,7 +165,12 @@ __global__ __launch_bounds__(256) void scan_step_kernel(fsc_selective_scan_args 
         float v = 0.f;
 #pragma unroll
         for (int i = 0; i < NS; ++i) {
-            h[r][i] = fmaf(__builtin_amdgcn_exp2f(delta * -__expf(al[r][i])), h[r][i], delta * kLn2 * u[r] * b[i]);
+            const float rate = __expf(al[r][i]);
+            al[r][i] = rate > FLT_MAX ? -FLT_MAX : -rate;
+        }
+#pragma unroll
+        for (int i = 0; i < NS; ++i) {
+            h[r][i] = fmaf(__builtin_amdgcn_exp2f(delta * al[r][i]), h[r][i], delta * kLn2 * u[r] * b[i]);
             if (i < have) v = fmaf(cc[i], h[r][i], v);
         }
         v = group_sum<L>(v);
@@ -197,6 +202,7 @@ int fsc_selective_scan_fwd(const fsc_selective_scan_args* args_host, fsc_stream_
     FSC_CHECK_ARG(a.length == 0 || (a.u && a.dt && a.b && a.c && a.y), "fsc_selective_scan_fwd: null u, dt, b, c or y");
     const ScanPlan p = scan_plan(a);
     FSC_CHECK_ARG(p.segments == 1 || a.workspace, "fsc_selective_scan_fwd: null workspace");
+    FSC_CHECK_ARG((long)a.batch * p.blocks * p.segments <= kMostBlocks, "fsc_selective_scan_fwd: batch * channels is too large");
     float* ends = reinterpret_cast<float*>(a.workspace);
     float* end_deltas = ends == nullptr ? nullptr : ends + (size_t)a.batch * p.segments * p.padded_channels() * p.padded_states();
     const dim3 grid((unsigned)((long)a.batch * p.blocks * p.segments));
@@ -225,6 +231,7 @@ int fsc_selective_scan_step(const fsc_selective_scan_args* args_host, fsc_stream
     // four channels a thread where that still leaves two workgroups a CU, else one
     const long fours = (long)a.batch * a.groups * ceil_div(p.group_channels, 4 * p.channels_block);
     const int r = fours >= 512 ? 4 : 1, group_blocks = ceil_div(p.group_channels, r * p.channels_block);
+    FSC_CHECK_ARG((long)a.batch * a.groups * group_blocks <= kMostBlocks, "fsc_selective_scan_step: batch * channels is too large");
     const dim3 grid((unsigned)((long)a.batch * a.groups * group_blocks));
     auto typed = [&](auto type) {
         using T = decltype(type);

@@ -387,7 +387,7 @@ __global__ __launch_bounds__(256) void scan_bwd_finish_kernel(fsc_selective_scan
     const long c = (long)(block / p.group_blocks) * p.group_channels + in_group;
     if (column < channels * sp) {
         const int s = (int)(column % sp);
-        if (s < a.states) a.da_log[c * a.states + s] = -expf(a.a_log[c * a.states + s]) * kLn2 * sum;         // dA / d a_log = A; delta over ln 2
+        if (s < a.states) a.da_log[c * a.states + s] = rate_of(a.a_log[c * a.states + s]) * kLn2 * sum;         // dA / d a_log = A; delta over ln 2
     } else if (column < channels * (sp + 1)) {
         if (a.dd != nullptr) a.dd[c] = sum;
     } else if (a.ddt_bias != nullptr) {
@@ -421,7 +421,7 @@ int fsc_selective_scan_bwd(const fsc_selective_scan_args* args_host, fsc_stream_
     const dim3 grid((unsigned)((long)a.batch * p.blocks * p.segments));
     const long rows = ((long)a.batch * a.length * a.groups * a.states + 255) / 256;
     const long columns = (p.padded_channels() * (p.padded_states() + 2) + 31) / 32;
-    FSC_CHECK_ARG(rows + columns < 0x7FFFFFFFL, "fsc_selective_scan_bwd: too large");
+    FSC_CHECK_ARG((long)a.batch * p.blocks * p.segments <= kMostBlocks && rows + columns <= kMostBlocks, "fsc_selective_scan_bwd: too large");
     auto typed = [&](auto type) {
         using T = decltype(type);
         if (a.batch > 0)

@@ -17,6 +17,7 @@ _DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 MAX_TAPS = 8
 MAX_STATES = 64
 _Tensor = torch.Tensor
+_moved_on = torch.autograd.graph.increment_version           # (a graph that saved the state in front of the step must not use it)
 
 
 def _fail(what, text, *args):
@@ -42,7 +43,7 @@ def _activation(what, name, t, shape, dtype, device):
         _check(what, name, t, shape, dtype, device)
     strides = t.stride()
     if (strides[-1] != 1 and shape[-1] > 1) or (len(strides) > 2 and strides[1] > 1 << 26):      # (the kernels step over frames in 32 bits)
-        t = t.contiguous()
+        t = t.clone(memory_format=torch.contiguous_format)       # (contiguous() keeps the strides of axes of length 1)
     return t
 
 
@@ -188,6 +189,7 @@ def causal_conv_step(x, window, weight, bias=None, activation="silu"):
     call("fsc_causal_conv_step",
          CausalConvArgs.packed(n, 1, d, taps, _DTYPES[x.dtype], int(activation is not None), x.data_ptr(), x.stride(0), 0, weight.data_ptr(),
                                _addr(bias), 0, window.data_ptr(), y.data_ptr(), 0, 0, 0, 0, 0, 0, 0, 0, 0, 0), stream_ptr())
+    _moved_on(window)
     return y
 
 
@@ -224,8 +226,8 @@ def _scan_forward(u, dt, a_log, b, c, d, z, dt_bias, initial, lengths, soft, wan
 class SelectiveScanFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, u, dt, a_log, b, c, d, z, dt_bias, initial, lengths, soft, want_final):
-        y, final, ctx.kept = _scan_forward(u, dt, a_log, b, c, d, z, dt_bias, initial, lengths, soft, want_final, keep=True)
-        ctx.save_for_backward(u, dt, a_log, b, c, d, z, dt_bias, initial, lengths)
+        y, final, kept = _scan_forward(u, dt, a_log, b, c, d, z, dt_bias, initial, lengths, soft, want_final, keep=True)
+        ctx.save_for_backward(u, dt, a_log, b, c, d, z, dt_bias, initial, lengths, kept)
         ctx.soft = soft
         ctx.set_materialize_grads(False)
         return y, final
@@ -235,12 +237,12 @@ class SelectiveScanFn(torch.autograd.Function):
     def backward(ctx, dy, dfinal):
         if dy is None and dfinal is None:
             return (None,) * 12
-        u, dt, a_log, b, c, d, z, dt_bias, initial, lengths = ctx.saved_tensors
+        u, dt, a_log, b, c, d, z, dt_bias, initial, lengths, kept = ctx.saved_tensors
         if dy is not None:
             dy = _activation("selective_scan", "the gradient", dy, u.shape, u.dtype, u.get_device())
         dfinal = None if dfinal is None else dfinal.contiguous()
         made = [None if t is None else t.new_empty(t.shape) for t in (u, dt, z, b, c, a_log, d, dt_bias, initial)]
-        same = (u, dt, a_log, b, c, d, z, dt_bias, ctx.soft, lengths, initial, None, None, ctx.kept)
+        same = (u, dt, a_log, b, c, d, z, dt_bias, ctx.soft, lengths, initial, None, None, kept)
         ws = _room(_lib.load().fsc_selective_scan_workspace_bytes(_scan_args(*same), 1), u)
         call("fsc_selective_scan_bwd", _scan_args(*same, ws, dy, dfinal, [_addr(t) for t in made]), stream_ptr())
         du, ddt, dz, db, dc, da, dd, dbias, di = made
@@ -299,4 +301,5 @@ def selective_scan_step(u, dt, a_log, b, c, state, d=None, z=None, dt_bias=None,
     _one_frame(what, u, dt, a_log, b, c, d, z, dt_bias)
     y = u.new_empty(u.shape)
     call("fsc_selective_scan_step", _scan_args(u, dt, a_log, b, c, d, z, dt_bias, int(bool(softplus)), None, None, y, state), stream_ptr())
+    _moved_on(state)
     return y

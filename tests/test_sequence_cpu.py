@@ -46,6 +46,16 @@ def test_scan_entry_points_refuse_bad_arguments(name):
         _refused(name, C.byref(_scan(**kw)), None, match=text)
 
 
+def test_launches_of_too_many_threads_are_refused():
+    _refused("fsc_causal_conv_fwd", C.byref(_conv(batch=2 ** 20, length=8, channels=2 ** 16, weight=64, x=64, y=64)), None, match="too large")
+    _refused("fsc_causal_conv_step", C.byref(_conv(batch=2 ** 20, channels=2 ** 16, weight=64, x=64, y=64, initial=64)), None, match="too large")
+    big = dict(batch=2 ** 16, channels=2 ** 13, states=64)
+    inputs = {key: 64 for key in ("u", "dt", "b", "c")}
+    _refused("fsc_selective_scan_fwd", C.byref(_scan(y=64, **inputs, **big)), None, match="too large")
+    grads = {key: 64 for key in ("checkpoints", "du", "ddt", "db", "dc", "da_log", "workspace")}
+    _refused("fsc_selective_scan_bwd", C.byref(_scan(**inputs, **grads, **big)), None, match="too large")
+
+
 def test_empty_calls_launch_nothing():
     lib = pkg.load_library()
     for kw in (dict(batch=0), dict(channels=0), dict(length=0)):

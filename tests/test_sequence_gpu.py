@@ -325,6 +325,44 @@ def test_frames_far_apart_are_copied():
     assert torch.equal(F.selective_scan(x, x, w.new_zeros(d, 3), rows, rows), F.selective_scan(x.contiguous(), x.contiguous(), w.new_zeros(d, 3), rows, rows))
 
 
+def test_one_frame_with_a_far_stride():
+    """An axis of length 1 may have any stride."""
+    gen = torch.Generator().manual_seed(5)
+    x, w = make((2, 1, 8), gen, torch.float32).to(DEV), make((8, 4), gen, torch.float32).to(DEV)
+    far = x.as_strided((2, 1, 8), (8, 2 ** 28, 1))
+    assert torch.equal(F.causal_conv(far, w), F.causal_conv(x, w))
+
+
+@pytest.mark.parametrize("n, t, s, lengths", [(2, 40, 16, [5, 33]), (2, 400, 5, [400, 77]), (1, 20, 64, None)])
+def test_states_that_forget_everything(n, t, s, lengths):
+    """exp(a_log) beyond fp32: such a state is delta u B of its frame alone, its rate's gradient 0, and padding behind the end changes nothing."""
+    d = 12
+    p, _, _ = scan_inputs(n, t, d, s, 1, "dzbi", torch.float32, 17)
+    p["a_log"][::2, 0] = 100.0
+    p["a_log"][1, :] = 90.0
+    gen = torch.Generator().manual_seed(18)
+    compare(scan_dev, scan_ref, p, lengths, [make((n, t, d), gen, torch.float32), make((n, d, s), gen, torch.float32)], t)
+
+
+def test_steps_mark_what_they_change():
+    """A graph that saved a state must notice that a step has moved it on."""
+    gen = torch.Generator().manual_seed(6)
+    x, w = make((2, 5, 8), gen, torch.float32).to(DEV), make((8, 4), gen, torch.float32).to(DEV)
+    window = make((2, 3, 8), gen, torch.float32).to(DEV)
+    y = F.causal_conv(x, w.requires_grad_(), initial=window)
+    with torch.no_grad():
+        F.causal_conv_step(x[:, 0], window, w)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.sum().backward()
+    u, a = x, make((8, 4), gen, torch.float32).to(DEV)
+    rows, state = make((2, 5, 4), gen, torch.float32).to(DEV), torch.zeros(2, 8, 4, device=DEV)
+    y = F.selective_scan(u, u, a.requires_grad_(), rows, rows, initial=state)
+    with torch.inference_mode():
+        F.selective_scan_step(u[:, 0], u[:, 0], a, rows[:, 0], rows[:, 0], state)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.sum().backward()
+
+
 def test_equal_inputs_give_equal_bits():
     p, lengths, cot = scan_inputs(6, 150, 200, 16, 2, "dzbil", torch.bfloat16, 9)
     dl = torch.tensor(lengths, dtype=torch.int32, device=DEV)
