@@ -53,29 +53,27 @@ __device__ __forceinline__ void frame(const fsc_causal_conv_args& a, int n, int 
 // Channels c .. c + V - 1 of the U frames from t, 0 <= t < len, as they lie in memory: U independent loads, which nothing waits for here.  Frames behind the
 // last are read from the last; the caller leaves them out.
 template <typename T, int V, int U>
-__device__ __forceinline__ void fetch(const void* base, long batch, long time, int n, int c, int t, int len, bool wide, int have, fsc::Pack<T, V> (&raw)[U]) {
+__device__ __forceinline__ void fetch(const void* base, long batch, long time, int n, int c, int t, int len, bool wide, int have, fsc::Raw<T, V> (&raw)[U]) {
     const int last = len - 1 - t;
     const T* p = reinterpret_cast<const T*>(base) + n * batch + t * time + c;
     if (wide) {
 #pragma unroll
-        for (int j = 0; j < U; ++j) raw[j] = fsc::load_pack<T, V>(p + (j < last ? j : last) * (int)time);
+        for (int j = 0; j < U; ++j) raw[j].wide(p + (j < last ? j : last) * (int)time);
     } else {
 #pragma unroll
-        for (int j = 0; j < U; ++j)
-#pragma unroll
-            for (int i = 0; i < V; ++i) raw[j].v[i] = p[(j < last ? j : last) * (int)time + (i < have ? i : have - 1)];
+        for (int j = 0; j < U; ++j) raw[j].narrow([&](int i) { return p + (j < last ? j : last) * (int)time + (i < have ? i : have - 1); });
     }
 }
 template <typename T, int V, int U>
-__device__ __forceinline__ void convert(const fsc::Pack<T, V> (&raw)[U], float (*out)[V]) {
+__device__ __forceinline__ void convert(const fsc::Raw<T, V> (&raw)[U], float (*out)[V]) {
 #pragma unroll
     for (int j = 0; j < U; ++j)
 #pragma unroll
-        for (int i = 0; i < V; ++i) out[j][i] = (float)raw[j].v[i];
+        for (int i = 0; i < V; ++i) out[j][i] = raw[j][i];
 }
 template <typename T, int V, int U>
 __device__ __forceinline__ void frames(const void* base, long batch, long time, int n, int c, int t, int len, bool wide, int have, float (*out)[V]) {
-    fsc::Pack<T, V> raw[U];
+    fsc::Raw<T, V> raw[U];
     fetch<T, V, U>(base, batch, time, n, c, t, len, wide, have, raw);
     convert<T, V, U>(raw, out);
 }
@@ -200,7 +198,7 @@ __global__ __launch_bounds__(kThreads) void conv_bwd_kernel(fsc_causal_conv_args
             for (int i = 0; i < V; ++i) dp[j][i] = 0.f;
         // frame t yields d pre[t]; with it frame t - (K - 1) has its gradient.  The next U frames are on their way while these are worked on:
         // with two waves a SIMD nothing else covers the loads (4 x 8191 x 2048 in bf16: 142 us without)
-        fsc::Pack<T, V> raw_x[U] = {}, raw_dy[U] = {};
+        fsc::Raw<T, V> raw_x[U] = {}, raw_dy[U] = {};
         auto ahead = [&](int t) {
             if (t < len) {       // (behind the end the last values stay, or the zeros: their gradient is 0 and must meet a number)
                 fetch<T, V, U>(a.x, a.x_batch, a.x_time, n, c, t, len, wide, have, raw_x);
@@ -378,10 +376,11 @@ Plan plan(const fsc_causal_conv_args& a) {
     return p;
 }
 
-// Blocks along the rows of the backward pass: enough for two blocks a CU, and no more partial sums than that.
+// Blocks along the rows of the backward pass: two blocks a CU, as many as the registers let in (4 x 8191 x 2048 in bf16: 115 us, with four
+// 120), and no more partial sums than that.
 int bwd_parts(const Plan& p) {
     const int across = fsc::ceil_div(p.groups, p.lanes), need = fsc::ceil_div(p.rows, kThreads / p.lanes);
-    const int most = fsc::ceil_div(1024, across);
+    const int most = fsc::ceil_div(512, across);
     return need < most ? (need > 0 ? need : 1) : most;
 }
 

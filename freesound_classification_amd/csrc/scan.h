@@ -112,9 +112,9 @@ __device__ __forceinline__ float sigmoid2(float v2) { return __builtin_amdgcn_rc
 // delta2 of E channels of a frame; 0 where the frame does not exist, so that the state passes it unchanged.  (The uniform choice stands outside the
 // loop: the E chains of transcendentals then run side by side.)
 template <int E, typename T>
-__device__ __forceinline__ void time_steps(const Pack<T, E>& dt, const float (&bias2)[E], bool soft, bool there, float (&raw)[E], float (&delta)[E]) {
+__device__ __forceinline__ void time_steps(const Raw<T, E>& dt, const float (&bias2)[E], bool soft, bool there, float (&raw)[E], float (&delta)[E]) {
 #pragma unroll
-    for (int i = 0; i < E; ++i) delta[i] = raw[i] = fmaf((float)dt.v[i], kLog2e, bias2[i]);
+    for (int i = 0; i < E; ++i) delta[i] = raw[i] = fmaf(dt[i], kLog2e, bias2[i]);
     if (soft) {
 #pragma unroll
         for (int i = 0; i < E; ++i) delta[i] = softplus2(raw[i]);
@@ -192,18 +192,17 @@ struct ScanFrames {
         base = reinterpret_cast<const char*>(reinterpret_cast<const T*>(ptr) + w.n * batch + w.c0);
         off = (uint32_t)w.te * (uint32_t)time + w.ce * (uint32_t)sizeof(T);
     }
-    __device__ __forceinline__ void fetch(const Place& w, int tile, int len, Pack<T, E>& out) const {
+    __device__ __forceinline__ void fetch(const Place& w, int tile, int len, Raw<T, E>& out) const {
         const int last = len - 1 - tile * kTile;
         const char* at = base + tile * kTile * time;
         const uint32_t o = w.te <= last ? off : (uint32_t)last * (uint32_t)time + w.ce * (uint32_t)sizeof(T);
         if (w.whole) {
-            out = load_pack<T, E>(reinterpret_cast<const T*>(at + o));
+            out.wide(reinterpret_cast<const T*>(at + o));
         } else {
-#pragma unroll
-            for (int i = 0; i < E; ++i) {
+            out.narrow([&](int i) {
                 const int c = w.ce + i < w.have ? w.ce + i : w.have - 1;
-                out.v[i] = *reinterpret_cast<const T*>(at + (o + (uint32_t)(c - w.ce) * (uint32_t)sizeof(T)));
-            }
+                return reinterpret_cast<const T*>(at + (o + (uint32_t)(c - w.ce) * (uint32_t)sizeof(T)));
+            });
         }
     }
 };

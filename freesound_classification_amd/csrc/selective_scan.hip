@@ -40,7 +40,7 @@ __global__ __launch_bounds__(256) void scan_fwd_kernel(fsc_selective_scan_args a
     }
     const ScanFrames<T, L, NS> u_rows(w, a.u, a.u_batch, a.u_time), dt_rows(w, a.dt, a.dt_batch, a.dt_time), z_rows(w, a.z, a.z_batch, a.z_time);
     ScanRows<T, L, NS> b_rows(w, a.b, a.b_batch, a.b_time, a.b_group, a.states), c_rows(w, a.c, a.c_batch, a.c_time, a.c_group, a.states);
-    Pack<T, E> u_next, dt_next, z_next;
+    Raw<T, E> u_next, dt_next, z_next;
     auto fetch = [&](int tile) {
         u_rows.fetch(w, tile, len, u_next);
         dt_rows.fetch(w, tile, len, dt_next);
@@ -49,15 +49,18 @@ __global__ __launch_bounds__(256) void scan_fwd_kernel(fsc_selective_scan_args a
         if (!ENDS) c_rows.fetch(w, tile, len);
     };
     if (w.first < w.work_end) fetch(w.first);
+    pin_all(h);
+    pin_all(bias);
+    pin_all(skip);
     for (int tile = w.first; tile < w.work_end; ++tile) {
         const int t = tile * kTile + w.te;
         float raw[E], delta[E];
         time_steps(dt_next, bias, a.softplus, t < len, raw, delta);
-        const Pack<T, E> u_now = u_next, z_now = z_next;
+        const Raw<T, E> u_now = u_next, z_now = z_next;
 #pragma unroll
         for (int i = 0; i < E; ++i) {
             s_delta[w.lds_row(i)][w.te] = delta[i];
-            s_du[w.lds_row(i)][w.te] = t < len ? delta[i] * (float)u_now.v[i] : 0.f;
+            s_du[w.lds_row(i)][w.te] = t < len ? delta[i] * u_now[i] : 0.f;
         }
         b_rows.stage(w, s_b, tile, len, a.states, kLn2);
         if constexpr (!ENDS) c_rows.stage(w, s_c, tile, len, a.states, 1.0f);
@@ -92,10 +95,10 @@ __global__ __launch_bounds__(256) void scan_fwd_kernel(fsc_selective_scan_args a
             if (t < a.length) {
                 float y[E];
 #pragma unroll
-                for (int i = 0; i < E; ++i) y[i] = fmaf(skip[i], (float)u_now.v[i], s_y[w.lds_row(i)][w.te]);
+                for (int i = 0; i < E; ++i) y[i] = fmaf(skip[i], u_now[i], s_y[w.lds_row(i)][w.te]);
                 if (a.z != nullptr) {
 #pragma unroll
-                    for (int i = 0; i < E; ++i) y[i] *= (float)z_now.v[i] * sigmoid_fast((float)z_now.v[i]);
+                    for (int i = 0; i < E; ++i) y[i] *= z_now[i] * sigmoid_fast(z_now[i]);
                 }
 #pragma unroll
                 for (int i = 0; i < E; ++i) y[i] = t < len ? y[i] : 0.f;

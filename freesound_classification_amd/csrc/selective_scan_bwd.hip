@@ -44,7 +44,7 @@ __global__ __launch_bounds__(256) void scan_bwd_ends_kernel(fsc_selective_scan_a
     for (int i = 0; i < E; ++i) bias[i] = a.dt_bias != nullptr && i < w.he ? a.dt_bias[w.c0 + w.ce + i] * kLog2e : 0.f;
     const ScanFrames<T, L, NS> dt_rows(w, a.dt, a.dt_batch, a.dt_time), z_rows(w, a.z, a.z_batch, a.z_time), dy_rows(w, a.dy, a.dy_batch, a.dy_time);
     ScanRows<T, L, NS> c_rows(w, a.c, a.c_batch, a.c_time, a.c_group, a.states);
-    Pack<T, E> dt_next, z_next, dy_next;
+    Raw<T, E> dt_next, z_next, dy_next;
     auto fetch = [&](int tile) {
         dt_rows.fetch(w, tile, len, dt_next);
         if (a.dy != nullptr) dy_rows.fetch(w, tile, len, dy_next);
@@ -52,16 +52,17 @@ __global__ __launch_bounds__(256) void scan_bwd_ends_kernel(fsc_selective_scan_a
         c_rows.fetch(w, tile, len);
     };
     if (w.first < w.work_end) fetch(w.work_end - 1);
+    pin_all(bias);
     for (int tile = w.work_end - 1; tile >= w.first; --tile) {
         const int t = tile * kTile + w.te;
         __syncthreads();
         float raw[E], delta[E], dyy[E];
         time_steps(dt_next, bias, a.softplus, t < len, raw, delta);
 #pragma unroll
-        for (int i = 0; i < E; ++i) dyy[i] = a.dy != nullptr ? (float)dy_next.v[i] : 0.f;
+        for (int i = 0; i < E; ++i) dyy[i] = a.dy != nullptr ? dy_next[i] : 0.f;
         if (a.z != nullptr) {
 #pragma unroll
-            for (int i = 0; i < E; ++i) dyy[i] *= (float)z_next.v[i] * sigmoid_fast((float)z_next.v[i]);
+            for (int i = 0; i < E; ++i) dyy[i] *= z_next[i] * sigmoid_fast(z_next[i]);
         }
 #pragma unroll
         for (int i = 0; i < E; ++i) {
@@ -153,7 +154,7 @@ __global__ __launch_bounds__(256, 2) void scan_bwd_kernel(fsc_selective_scan_arg
     const ScanFrames<T, L, NS> u_rows(w, a.u, a.u_batch, a.u_time), dt_rows(w, a.dt, a.dt_batch, a.dt_time), z_rows(w, a.z, a.z_batch, a.z_time),
         dy_rows(w, a.dy, a.dy_batch, a.dy_time);
     ScanRows<T, L, NS> b_rows(w, a.b, a.b_batch, a.b_time, a.b_group, a.states), c_rows(w, a.c, a.c_batch, a.c_time, a.c_group, a.states);
-    Pack<T, E> u_next, dt_next, z_next, dy_next;
+    Raw<T, E> u_next, dt_next, z_next, dy_next;
     Pack<float, NS> h_next;
     auto fetch = [&](int tile) {
         u_rows.fetch(w, tile, len, u_next);
@@ -174,14 +175,17 @@ __global__ __launch_bounds__(256, 2) void scan_bwd_kernel(fsc_selective_scan_arg
         for (int j = threadIdx.x; j < kTile * 2 * SP; j += 256) ws[at.rows + w.rows(p, tile) + j] = 0.f;
     }
     if (w.first < w.work_end) fetch(w.work_end - 1);
+    pin_all(e);
+    pin_all(bias);
+    pin_all(skip);
     for (int tile = w.work_end - 1; tile >= w.first; --tile) {
         const int t = tile * kTile + w.te;
-        const Pack<T, E> u_now = u_next;
+        const Raw<T, E> u_now = u_next;
         float raw[E], delta[E], dyy[E], sig[E], gz[E], h[NS], hp[kTile][NS], ex[kTile][NS];
         time_steps(dt_next, bias, a.softplus, t < len, raw, delta);
 #pragma unroll
         for (int i = 0; i < E; ++i) {
-            dyy[i] = t < len && i < w.he && a.dy != nullptr ? (float)dy_next.v[i] : 0.f;
+            dyy[i] = t < len && i < w.he && a.dy != nullptr ? dy_next[i] : 0.f;
             sig[i] = 1.0f;
             gz[i] = 0.f;
         }
@@ -192,7 +196,7 @@ __global__ __launch_bounds__(256, 2) void scan_bwd_kernel(fsc_selective_scan_arg
         if (a.z != nullptr) {
 #pragma unroll
             for (int i = 0; i < E; ++i) {
-                const float z = t < len ? (float)z_next.v[i] : 0.f, s = sigmoid_fast(z), zs = z * s;
+                const float z = t < len ? z_next[i] : 0.f, s = sigmoid_fast(z), zs = z * s;
                 gz[i] = dyy[i] * (fmaf(-zs, s, zs) + s);
                 dyy[i] *= zs;
             }
@@ -201,7 +205,7 @@ __global__ __launch_bounds__(256, 2) void scan_bwd_kernel(fsc_selective_scan_arg
         for (int i = 0; i < E; ++i) {
             s_delta[w.lds_row(i)][w.te] = delta[i];
             // (a channel that does not exist must not enter the sums over channels)
-            s_du[w.lds_row(i)][w.te] = t < len && i < w.he ? delta[i] * (float)u_now.v[i] : 0.f;
+            s_du[w.lds_row(i)][w.te] = t < len && i < w.he ? delta[i] * u_now[i] : 0.f;
             s_dyy[w.lds_row(i)][w.te] = dyy[i];
         }
         store_row<E>(s_sig[threadIdx.x], true, E, sig);
@@ -293,7 +297,7 @@ __global__ __launch_bounds__(256, 2) void scan_bwd_kernel(fsc_selective_scan_arg
 #pragma unroll
             for (int i = 0; i < E; ++i) {
                 const int r = w.lds_row(i);
-                const float u = t < len ? (float)u_now.v[i] : 0.f, gb = s_gb[r][w.te], ga = s_ga[r][w.te], dyy = s_dyy[r][w.te];
+                const float u = t < len ? u_now[i] : 0.f, gb = s_gb[r][w.te], ga = s_ga[r][w.te], dyy = s_dyy[r][w.te];
                 du_out[i] = fmaf(s_delta[r][w.te], gb, skip[i] * dyy);          // (B was staged times ln 2, delta over it)
                 ddt_out[i] = fmaf(u * kLog2e, gb, ga) * sig[i];
                 dz_out[i] = gz[i] * fmaf(skip[i], u, s_yh[r][w.te]);

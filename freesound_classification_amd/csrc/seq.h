@@ -29,6 +29,41 @@ __device__ __forceinline__ void store_pack(T* p, const Pack<T, V>& v) {
     *reinterpret_cast<typename Word<sizeof(T) * V>::type*>(p) = __builtin_bit_cast(typename Word<sizeof(T) * V>::type, v);
 }
 
+// V consecutive values on their way from memory, as the 32-bit words that hold them; converted where they are used.  (Held as values, those of a
+// wide load would be taken apart where the wide and the narrow path meet, right behind the load, and so would wait for it there.)
+template <typename T, int V>
+struct Raw {
+    uint32_t w[(V * sizeof(T) + 3) / 4];
+    __device__ __forceinline__ float operator[](int i) const {
+        if constexpr (sizeof(T) == 4) {
+            const uint32_t word = w[i];
+            return __builtin_bit_cast(float, word);
+        } else {
+            const uint16_t half = (uint16_t)(w[i / 2] >> (16 * (i & 1)));
+            return (float)__builtin_bit_cast(T, half);
+        }
+    }
+    __device__ __forceinline__ void wide(const T* p) {
+        const auto word = *reinterpret_cast<const typename Word<sizeof(T) * V>::type*>(p);
+        if constexpr (sizeof(T) * V < 4) w[0] = word;
+        else *this = __builtin_bit_cast(Raw, word);
+    }
+    // from(i): the address of the i-th value
+    template <typename From>
+    __device__ __forceinline__ void narrow(From from) {
+#pragma unroll
+        for (int i = 0; i < (int)(sizeof(w) / 4); ++i) {
+            if constexpr (sizeof(T) == 4) {
+                w[i] = *reinterpret_cast<const uint32_t*>(from(i));
+            } else {
+                w[i] = *reinterpret_cast<const uint16_t*>(from(2 * i));
+                if (2 * i + 1 < V) w[i] |= (uint32_t)*reinterpret_cast<const uint16_t*>(from(2 * i + 1)) << 16;
+            }
+            asm volatile("" : "+v"(w[i]));
+        }
+    }
+};
+
 // V consecutive values at `p` as floats: one wide load where `wide`, else one by one and only the first `have` (the others are 0).
 template <int V, typename T>
 __device__ __forceinline__ void load_row(const T* p, bool wide, int have, float (&out)[V]) {
@@ -65,6 +100,13 @@ __device__ __forceinline__ float dpp(float v) {
 // The value is there from here on: sums that nothing reads for a while are otherwise put off, with all their terms kept in registers until
 // then, and lane exchanges end up under a mask, where they cannot be part of the addition.
 __device__ __forceinline__ void pin(float& v) { asm volatile("" : "+v"(v)); }
+
+// ... of an array; in front of a loop: what was loaded there is waited for there, not at its first use inside, behind the loop's own loads.
+template <int N>
+__device__ __forceinline__ void pin_all(float (&v)[N]) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) pin(v[i]);
+}
 
 // The sum over aligned groups of L <= 16 lanes, in every lane of the group.
 template <int L>
