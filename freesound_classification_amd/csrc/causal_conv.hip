@@ -1,11 +1,12 @@
 // Short causal convolution along time, one filter of K <= 8 taps a channel, SiLU behind it (the sequence head's local mixing).
 //   pre[t] = bias + sum_k w[k] xin[t + k],  xin = [K - 1 frames before | x];  y = silu(pre)
-// Bound: HBM (two passes over the frames forward, three backward), K multiply-adds and one exponential a value.  So each thread owns
-// four channels and walks a strip of frames with the filter's window in registers: every frame is read
-// once but for the K - 1 at a strip's ends, neighbouring threads read neighbouring channels.  Frames are taken eight at a time, all
-// their loads issued before the first is used.
+// Bound: HBM (two passes over the frames forward, three backward), K multiply-adds and one exponential a value.  So each thread owns four channels
+// and walks a strip of frames with the filter's window in registers: every frame is read once but for the K - 1 at a strip's ends,
+// neighbouring threads read neighbouring channels.  Frames are taken eight at a time, all their loads issued before the first is used.
 // Backward: the strip recomputes pre (cheaper than keeping it) and runs K - 1 frames past its end; dw / db are summed in registers, over
 // the block's strips through LDS, over blocks by a second launch in a fixed order: equal inputs give equal bits.
+// 4 x 8191 x 2048 in bf16, ragged (80 % of the frames), x a half of a wider tensor: forward 53 us (4.5 TB/s, what a copy of this size reaches), backward 93
+// (3.7 TB/s: two waves a SIMD, the window, its gradient and the filters' sums fill the registers).  128 x 53 x 256 in fp32: 6.5 and 17 us.
 #include <type_traits>
 
 #include "seq.h"
@@ -197,7 +198,7 @@ __global__ __launch_bounds__(kThreads) void conv_bwd_kernel(fsc_causal_conv_args
 #pragma unroll
             for (int i = 0; i < V; ++i) dp[j][i] = 0.f;
         // frame t yields d pre[t]; with it frame t - (K - 1) has its gradient.  The next U frames are on their way while these are worked on:
-        // with two waves a SIMD nothing else covers the loads (4 x 8191 x 2048 in bf16: 142 us without)
+        // with two waves a SIMD nothing else covers the loads (4 x 8191 x 2048 in bf16: 97 us, 120 where each load was waited for at once)
         fsc::Raw<T, V> raw_x[U] = {}, raw_dy[U] = {};
         auto ahead = [&](int t) {
             if (t < len) {       // (behind the end the last values stay, or the zeros: their gradient is 0 and must meet a number)
@@ -259,6 +260,13 @@ __global__ __launch_bounds__(kThreads) void conv_bwd_kernel(fsc_causal_conv_args
                         load_row<V>(reinterpret_cast<const T*>(a.dfinal) + ((long)n * (K - 1) + f) * a.channels + c, wide, have, more);
 #pragma unroll
                         for (int i = 0; i < V; ++i) dx[i] += more[i];
+                    }
+                }
+                if (j == U - 1) {                    // (95 us for 97)
+#pragma unroll
+                    for (int q = 0; q < U; ++q) {
+                        raw_x[q].arrived();
+                        raw_dy[q].arrived();
                     }
                 }
                 if (at >= t0 && at < t1) store_row<V>(out + j * a.channels, wide, have, dx);
@@ -376,7 +384,7 @@ Plan plan(const fsc_causal_conv_args& a) {
     return p;
 }
 
-// Blocks along the rows of the backward pass: two blocks a CU, as many as the registers let in (4 x 8191 x 2048 in bf16: 115 us, with four
+// Blocks along the rows of the backward pass: two blocks a CU, as many as the registers let in (4 x 8191 x 2048 in bf16: 116 us, with four
 // 120), and no more partial sums than that.
 int bwd_parts(const Plan& p) {
     const int across = fsc::ceil_div(p.groups, p.lanes), need = fsc::ceil_div(p.rows, kThreads / p.lanes);

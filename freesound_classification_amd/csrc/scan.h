@@ -44,8 +44,8 @@ inline ScanPlan scan_plan(const fsc_selective_scan_args& a) {
     p.group_blocks = ceil_div(p.group_channels, p.channels_block);
     p.blocks = a.groups * p.group_blocks;
     p.tiles = ceil_div(a.length, kTile);
-    // 1024 workgroups are four waves a SIMD (a long training step, 8 x 2048 frames of 1024 channels, forward + its ends | backward + its ends:
-    // 512: 190 | 358 us, 1024: 133 | 309, 2048: 143 | 321).  Segments double the exponentials, so half of that is enough not to cut (a batch of 128 x
+    // 1024 workgroups are four waves a SIMD (a long training step, 8 x 2048 frames of 1024 channels, forward + its ends | backward + its ends,
+    // when a tile's loads were still waited for at once: 512: 190 | 358 us, 1024: 133 | 309, 2048: 143 | 321).  Segments double the exponentials, so half of that is enough not to cut (a batch of 128 x
     // 53 frames of 256 channels, 512 workgroups: 19 | 39 us whole, 31 | 62 cut in two).
     const long have = (long)a.batch * p.blocks, wanted = 1024;
     p.segments = 1;
@@ -215,7 +215,7 @@ struct ScanRows {
     const char* base;
     long time;
     uint32_t off[R], col[R];
-    T v[R];
+    Raw<T, 1> v[R];
     __device__ ScanRows(const Place& w, const void* ptr, long batch, long time_, long group, int states) : time(time_ * (long)sizeof(T)) {
         base = reinterpret_cast<const char*>(reinterpret_cast<const T*>(ptr) + w.n * batch + w.group * group);
 #pragma unroll
@@ -231,12 +231,12 @@ struct ScanRows {
         const char* at = base + tile * kTile * time;
 #pragma unroll
         for (int j = 0; j < R; ++j)
-            v[j] = *reinterpret_cast<const T*>(at + (row(w, j) <= last ? off[j] : (uint32_t)last * (uint32_t)time + col[j]));
+            v[j].wide(reinterpret_cast<const T*>(at + (row(w, j) <= last ? off[j] : (uint32_t)last * (uint32_t)time + col[j])));
     }
     __device__ __forceinline__ void stage(const Place& w, float (*to)[Place::SP], int tile, int len, int states, float unit) const {
 #pragma unroll
         for (int j = 0; j < R; ++j)
-            if (w.bc_mine(j)) to[w.bc_row(j)][w.bc_state(j)] = tile * kTile + w.bc_row(j) < len && w.bc_state(j) < states ? (float)v[j] * unit : 0.f;
+            if (w.bc_mine(j)) to[w.bc_row(j)][w.bc_state(j)] = tile * kTile + w.bc_row(j) < len && w.bc_state(j) < states ? v[j][0] * unit : 0.f;
     }
 };
 
@@ -256,21 +256,42 @@ __device__ __forceinline__ float rate_of(float a_log) {
 // A of the lane's states, 0 for states that do not exist.
 template <int L, int NS>
 __device__ __forceinline__ void scan_rates(const fsc_selective_scan_args& a, const ScanPlace<L, NS>& w, float (&rate)[NS]) {
+    // (all the loads first, from places that exist: a load under a condition is waited for before the next)
 #pragma unroll
     for (int i = 0; i < NS; ++i) {
         const int s = w.sg * NS + i;
-        rate[i] = w.real && s < a.states ? rate_of(a.a_log[(long)w.channel * a.states + s]) : 0.f;
+        rate[i] = a.a_log[(long)w.channel * a.states + (s < a.states ? s : 0)];
     }
+#pragma unroll
+    for (int i = 0; i < NS; ++i) rate[i] = w.real && w.sg * NS + i < a.states ? rate_of(rate[i]) : 0.f;
 }
 
 // The lane's states of a (batch, channels, states) tensor, zeros without one.
 template <int L, int NS>
 __device__ __forceinline__ void scan_state(const fsc_selective_scan_args& a, const ScanPlace<L, NS>& w, const float* from, float (&h)[NS]) {
 #pragma unroll
+    for (int i = 0; i < NS; ++i) h[i] = 0.f;
+    if (from == nullptr) return;
+#pragma unroll
     for (int i = 0; i < NS; ++i) {
         const int s = w.sg * NS + i;
-        h[i] = from != nullptr && w.real && s < a.states ? from[((long)w.n * a.channels + w.channel) * a.states + s] : 0.f;
+        h[i] = from[((long)w.n * a.channels + w.channel) * a.states + (s < a.states ? s : 0)];
     }
+#pragma unroll
+    for (int i = 0; i < NS; ++i) h[i] = w.real && w.sg * NS + i < a.states ? h[i] : 0.f;
+}
+
+// E elementwise channels of a (channels) parameter, zeros without one and where a channel does not exist.
+template <int L, int NS>
+__device__ __forceinline__ void scan_param(const ScanPlace<L, NS>& w, const float* from, float (&out)[ScanPlace<L, NS>::E]) {
+    constexpr int E = ScanPlace<L, NS>::E;
+#pragma unroll
+    for (int i = 0; i < E; ++i) out[i] = 0.f;
+    if (from == nullptr) return;
+#pragma unroll
+    for (int i = 0; i < E; ++i) out[i] = from[w.c0 + (i < w.he ? w.ce + i : 0)];
+#pragma unroll
+    for (int i = 0; i < E; ++i) out[i] = i < w.he ? out[i] : 0.f;
 }
 
 // fn(lanes, per_lane) with the plan's two constants as types

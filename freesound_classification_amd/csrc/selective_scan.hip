@@ -33,11 +33,10 @@ __global__ __launch_bounds__(256) void scan_fwd_kernel(fsc_selective_scan_args a
         }
     }
     float bias[E], skip[E];
+    scan_param(w, a.dt_bias, bias);
+    scan_param(w, ENDS ? nullptr : a.d, skip);
 #pragma unroll
-    for (int i = 0; i < E; ++i) {
-        bias[i] = a.dt_bias != nullptr && i < w.he ? a.dt_bias[w.c0 + w.ce + i] * kLog2e : 0.f;
-        skip[i] = !ENDS && a.d != nullptr && i < w.he ? a.d[w.c0 + w.ce + i] : 0.f;
-    }
+    for (int i = 0; i < E; ++i) bias[i] *= kLog2e;
     const ScanFrames<T, L, NS> u_rows(w, a.u, a.u_batch, a.u_time), dt_rows(w, a.dt, a.dt_batch, a.dt_time), z_rows(w, a.z, a.z_batch, a.z_time);
     ScanRows<T, L, NS> b_rows(w, a.b, a.b_batch, a.b_time, a.b_group, a.states), c_rows(w, a.c, a.c_batch, a.c_time, a.c_group, a.states);
     Raw<T, E> u_next, dt_next, z_next;

@@ -40,8 +40,9 @@ __global__ __launch_bounds__(256) void scan_bwd_ends_kernel(fsc_selective_scan_a
     float rate[NS], e[NS] = {}, sum = 0.f;
     scan_rates(a, w, rate);
     float bias[E];
+    scan_param(w, a.dt_bias, bias);
 #pragma unroll
-    for (int i = 0; i < E; ++i) bias[i] = a.dt_bias != nullptr && i < w.he ? a.dt_bias[w.c0 + w.ce + i] * kLog2e : 0.f;
+    for (int i = 0; i < E; ++i) bias[i] *= kLog2e;
     const ScanFrames<T, L, NS> dt_rows(w, a.dt, a.dt_batch, a.dt_time), z_rows(w, a.z, a.z_batch, a.z_time), dy_rows(w, a.dy, a.dy_batch, a.dy_time);
     ScanRows<T, L, NS> c_rows(w, a.c, a.c_batch, a.c_time, a.c_group, a.states);
     Raw<T, E> dt_next, z_next, dy_next;
@@ -146,16 +147,15 @@ __global__ __launch_bounds__(256, 2) void scan_bwd_kernel(fsc_selective_scan_arg
         for (int i = 0; i < NS; ++i) e[i] = fmaf(__builtin_amdgcn_exp2f(rate[i] * ds), e[i], more[i]);
     }
     float bias[E], skip[E], dskip[E] = {}, dbias[E] = {};
+    scan_param(w, a.dt_bias, bias);
+    scan_param(w, a.d, skip);
 #pragma unroll
-    for (int i = 0; i < E; ++i) {
-        bias[i] = a.dt_bias != nullptr && i < w.he ? a.dt_bias[w.c0 + w.ce + i] * kLog2e : 0.f;
-        skip[i] = a.d != nullptr && i < w.he ? a.d[w.c0 + w.ce + i] : 0.f;
-    }
+    for (int i = 0; i < E; ++i) bias[i] *= kLog2e;
     const ScanFrames<T, L, NS> u_rows(w, a.u, a.u_batch, a.u_time), dt_rows(w, a.dt, a.dt_batch, a.dt_time), z_rows(w, a.z, a.z_batch, a.z_time),
         dy_rows(w, a.dy, a.dy_batch, a.dy_time);
     ScanRows<T, L, NS> b_rows(w, a.b, a.b_batch, a.b_time, a.b_group, a.states), c_rows(w, a.c, a.c_batch, a.c_time, a.c_group, a.states);
     Raw<T, E> u_next, dt_next, z_next, dy_next;
-    Pack<float, NS> h_next;
+    Raw<float, NS> h_next;
     auto fetch = [&](int tile) {
         u_rows.fetch(w, tile, len, u_next);
         dt_rows.fetch(w, tile, len, dt_next);
@@ -163,7 +163,7 @@ __global__ __launch_bounds__(256, 2) void scan_bwd_kernel(fsc_selective_scan_arg
         if (a.z != nullptr) z_rows.fetch(w, tile, len, z_next);
         b_rows.fetch(w, tile, len);
         c_rows.fetch(w, tile, len);
-        h_next = load_pack<float, NS>(a.checkpoints + w.kept(p, tile));
+        h_next.wide(a.checkpoints + w.kept(p, tile));
     };
     for (int tile = w.zero_first; tile < w.zero_end; ++tile) {
         float zero[E] = {};
@@ -213,7 +213,7 @@ __global__ __launch_bounds__(256, 2) void scan_bwd_kernel(fsc_selective_scan_arg
         b_rows.stage(w, s_b, tile, len, a.states, kLn2);
         c_rows.stage(w, s_c, tile, len, a.states, 1.0f);
 #pragma unroll
-        for (int i = 0; i < NS; ++i) h[i] = h_next.v[i];
+        for (int i = 0; i < NS; ++i) h[i] = h_next[i];
         __syncthreads();
         if (tile > w.first) fetch(tile - 1);
 #pragma unroll

@@ -48,6 +48,11 @@ struct Raw {
         if constexpr (sizeof(T) * V < 4) w[0] = word;
         else *this = __builtin_bit_cast(Raw, word);
     }
+    // Waits for the load here.  Loads and stores are counted together, in order: in front of stores, a load is not held up by them.
+    __device__ __forceinline__ void arrived() {
+#pragma unroll
+        for (int i = 0; i < (int)(sizeof(w) / 4); ++i) asm volatile("" : "+v"(w[i]));
+    }
     // from(i): the address of the i-th value
     template <typename From>
     __device__ __forceinline__ void narrow(From from) {
@@ -59,8 +64,8 @@ struct Raw {
                 w[i] = *reinterpret_cast<const uint16_t*>(from(2 * i));
                 if (2 * i + 1 < V) w[i] |= (uint32_t)*reinterpret_cast<const uint16_t*>(from(2 * i + 1)) << 16;
             }
-            asm volatile("" : "+v"(w[i]));
         }
+        arrived();
     }
 };
 
