@@ -2,7 +2,9 @@
 // held in 8 bits changes with the last bit, and a plain evaluation of the same formulas then holds the same bits):
 //   g = grad * grad_scale;  m = m beta1 + g (1 - beta1);  v = v beta2 + (g g)(1 - beta2);  r = sqrt(v)
 //   p = p decay - (m / (r inv_root + eps)) step_size
-// Bound: HBM.  32-bit moments: 28 bytes a parameter in fp32 (p, g, m, v read; p, m, v written); 8-bit moments: 16.
+// Bound: HBM.  32-bit moments: 28 bytes a parameter in fp32 (p, g, m, v read; p, m, v written); 8-bit moments: 16, 10 in bf16.
+// 21 M parameters in 141 tensors: 107 us with 32 bits (5.5 TB/s; part of it stays in the last-level cache), 75 with 8; 200 M in bf16 with 8 bits: 500 us
+// (4.1 TB/s, and some 75 vector instructions an element).
 //
 // 8-bit moments.  m and r = sqrt(v) (half the decades of v) are held as e4m3 values of x / scale, scale = the largest |x| of 256
 // consecutive elements / 448.  Rounding to nearest would freeze them: beta2 = 0.999 moves v by 0.1 % a step and half a step of e4m3 is

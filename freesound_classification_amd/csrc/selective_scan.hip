@@ -124,7 +124,8 @@ __global__ __launch_bounds__(256) void scan_fwd_kernel(fsc_selective_scan_args a
 }
 
 // One frame.  Bound: the state, read and written once, in 16-byte accesses; L lanes a channel as in the scan.  A workgroup takes R x CB
-// channels of one sequence, each thread R of them with all their loads in flight and one read of B and C.
+// channels of one sequence, each thread R of them with all their loads in flight and one read of B and C.  256 sequences x 2048 channels x 64 states:
+// 58 us, 4.7 TB/s; one of 256 channels: 2.8 us.
 template <typename T, int L, int NS, int R>
 __global__ __launch_bounds__(256) void scan_step_kernel(fsc_selective_scan_args a, int group_channels, int group_blocks, int wide) {
     constexpr int CB = 256 / L;
