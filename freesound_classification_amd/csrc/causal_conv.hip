@@ -387,6 +387,7 @@ Plan plan(const fsc_causal_conv_args& a) {
 // Blocks along the rows of the backward pass: two blocks a CU, as many as the registers let in (4 x 8191 x 2048 in bf16: 116 us, with four
 // 120), and no more partial sums than that.
 int bwd_parts(const Plan& p) {
+    if (p.groups == 0) return 1;                 // no channels: nothing is launched
     const int across = fsc::ceil_div(p.groups, p.lanes), need = fsc::ceil_div(p.rows, kThreads / p.lanes);
     const int most = fsc::ceil_div(512, across);
     return need < most ? (need > 0 ? need : 1) : most;

@@ -52,7 +52,7 @@ inline ScanPlan scan_plan(const fsc_selective_scan_args& a) {
     // 53 frames of 256 channels, 512 workgroups: 19 | 39 us whole, 31 | 62 cut in two).
     const long have = (long)a.batch * p.blocks, wanted = 1024;
     p.segments = 1;
-    if (have * 2 < wanted && p.tiles >= 4) {
+    if (have > 0 && have * 2 < wanted && p.tiles >= 4) {        // (no sequences or no channels: nothing to cut)
         long want = (wanted + have - 1) / have, most = p.tiles / 2;
         if (most > 32) most = 32;
         p.segments = (int)(want < most ? want : most);
