@@ -414,21 +414,21 @@ int fsc_selective_scan_bwd(const fsc_selective_scan_args* args_host, fsc_stream_
     const char* why = scan_bad(args_host);
     FSC_CHECK_ARG(why == nullptr, "fsc_selective_scan_bwd: %s", why);
     const fsc_selective_scan_args& a = *args_host;
-    if (a.channels == 0) return 0;
     const ScanPlan p = scan_plan(a);
     const Carve at(a, p);
-    FSC_CHECK_ARG(a.da_log && (a.workspace || at.bytes == 0), "fsc_selective_scan_bwd: null da_log or workspace");
-    FSC_CHECK_ARG(a.batch == 0 || a.length == 0 ||
-                      (a.u && a.dt && a.b && a.c && a.checkpoints && a.du && a.ddt && a.db && a.dc && (a.z == nullptr || a.dz)),
+    FSC_CHECK_ARG(a.channels == 0 || (a.da_log && (a.workspace || at.bytes == 0)), "fsc_selective_scan_bwd: null da_log or workspace");
+    FSC_CHECK_ARG(a.batch == 0 || a.length == 0 || (a.db && a.dc && (a.channels == 0 || (a.u && a.dt && a.b && a.c && a.checkpoints && a.du && a.ddt &&
+                                                                                        (a.z == nullptr || a.dz)))),
                   "fsc_selective_scan_bwd: null input or gradient");
     float* ws = reinterpret_cast<float*>(a.workspace);
     const dim3 grid((unsigned)((long)a.batch * p.blocks * p.segments));
     const long rows = ((long)a.batch * a.length * a.groups * a.states + 255) / 256;
     const long columns = (p.padded_channels() * (p.padded_states() + 2) + 31) / 32;
     FSC_CHECK_ARG((long)a.batch * p.blocks * p.segments <= kMostBlocks && rows + columns <= kMostBlocks, "fsc_selective_scan_bwd: too large");
+    if (rows + columns == 0) return 0;
     auto typed = [&](auto type) {
         using T = decltype(type);
-        if (a.batch > 0)
+        if (a.batch > 0 && a.channels > 0)               // (without channels db and dc are still there: sums over nothing)
             with_scan_shape(p, [&](auto lanes, auto per) {
                 constexpr int L = decltype(lanes)::value, NS = decltype(per)::value;
                 if (p.segments > 1)
