@@ -1,0 +1,108 @@
+"""AdamW's host side without a device: what a step looks at before it launches.  The launch itself is replaced by one that notes its table;
+tensors in host memory stand for those of device 0."""
+import ctypes as C
+
+import numpy as np
+import pytest
+import torch
+
+from freesound_classification_amd import _lib
+from freesound_classification_amd.ops import training
+from freesound_classification_amd.ops.training import FusedAdamW
+
+
+@pytest.fixture
+def launches(monkeypatch):
+    """Every launch: (rows of the tensor table, arguments)."""
+    made = []
+
+    def note(name, table, n, *args):
+        made.append((np.ctypeslib.as_array(C.cast(table, C.POINTER(C.c_int64)), (n, 8)).copy(), args))
+
+    elsewhere = set()
+    monkeypatch.setattr(training, "call", note)
+    monkeypatch.setattr(training, "stream_ptr", lambda: 0)
+    monkeypatch.setattr(training, "_device_number", lambda t: 1 if id(t) in elsewhere else 0)
+    monkeypatch.setattr(_lib, "_get_device", lambda: 0)
+    made_on = made, elsewhere
+    return made_on
+
+
+def _parameters(*sizes, dtype=torch.float32):
+    params = [torch.nn.Parameter(torch.ones(size, dtype=dtype)) for size in sizes]
+    for p in params:
+        p.grad = torch.ones_like(p)
+    return params
+
+
+KEYS = {32: ["exp_avg", "exp_avg_sq"], 8: ["exp_avg", "exp_avg_sq_root", "exp_avg_scale", "exp_avg_sq_root_scale"]}
+
+
+def _wrong(good):
+    """What must not be launched in the place of a good moment: another size, another type, strides, not a tensor, nothing."""
+    n = good.numel()
+    other = torch.bfloat16 if good.dtype == torch.float32 else torch.uint8
+    wide = torch.zeros(2 * n, dtype=good.dtype)
+    return [good[:n - 1], torch.zeros(n + 1, dtype=good.dtype), torch.zeros(n, dtype=other), torch.zeros(n, dtype=torch.float64), wide[::2],
+            torch.zeros(1, dtype=good.dtype).expand(n), good.numpy(force=True) if good.dtype == torch.float32 else None, None]
+
+
+@pytest.mark.parametrize("bits, key", [(bits, key) for bits in (32, 8) for key in KEYS[bits]])
+def test_every_moment_is_looked_at(launches, bits, key):
+    made, elsewhere = launches
+    params = _parameters(600, 300)
+    opt = FusedAdamW(params, state_bits=bits)
+    opt.step()
+    assert len(made) == 1 and made[0][0][:, 6].tolist() == [600, 300]
+    st = opt.state[params[0]]
+    held = [opt.state[p][k].data_ptr() for p in params for k in KEYS[bits]]
+    assert made[0][0][:, 2:2 + len(KEYS[bits])].reshape(-1).tolist() == held
+    good = st[key]
+    for bad in _wrong(good):
+        st[key] = bad
+        with pytest.raises(_lib.FscError, match="moments"):
+            opt.step()
+    del st[key]
+    with pytest.raises(_lib.FscError, match="moments"):
+        opt.step()
+    st[key] = good
+    elsewhere.add(id(good))
+    with pytest.raises(_lib.FscError, match="device"):
+        opt.step()
+    elsewhere.clear()
+    assert len(made) == 1 and all(opt.state[p]["step"] == 1 for p in params)
+    opt.step()
+    assert len(made) == 2 and all(opt.state[p]["step"] == 2 for p in params)
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_no_moments_are_made_where_others_are_refused(launches, bits):
+    made, _ = launches
+    params = _parameters(600, 300)
+    params[1].grad = None
+    opt = FusedAdamW(params, state_bits=bits)
+    opt.step()
+    params[1].grad = torch.ones(300)
+    opt.state[params[0]]["exp_avg"] = torch.zeros(599)
+    with pytest.raises(_lib.FscError, match="moments"):
+        opt.step()
+    assert not opt.state[params[1]] and len(made) == 1
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_late_parameters_and_types_get_their_own_launches(launches, bits):
+    """What the table of a launch holds: tensors of one type and step count each, with their own moments and salts."""
+    made, _ = launches
+    params = _parameters(10, 20) + _parameters(30, dtype=torch.bfloat16) + _parameters(0, 513)
+    params[1].grad = None
+    opt = FusedAdamW(params, state_bits=bits, seed=5)
+    opt.step()
+    params[1].grad = torch.ones(20)
+    opt.step()
+    tables = [sorted(zip(t[:, 6].tolist(), t[:, 7].tolist())) for t, _ in made]
+    assert tables == [[(0, 8), (10, 5), (513, 9)], [(30, 7)], [(0, 8), (10, 5), (513, 9)], [(20, 6)], [(30, 7)]]
+    for table, _ in made[2:]:
+        for row in table:
+            p = next(p for p in params if p.numel() == row[6])
+            assert row[:2 + len(KEYS[bits])].tolist() == [p.data_ptr(), p.grad.data_ptr()] + [opt.state[p][k].data_ptr() for k in KEYS[bits]]
+    assert [opt.state[p]["step"] for p in params] == [2, 1, 2, 2, 2]
