@@ -300,25 +300,32 @@ class FusedAdamW(Optimizer):
         return out
 
     def load_state_dict(self, state_dict):
-        """Like torch's, but the moments keep the types they are held in (torch casts floating state to the parameter's type)."""
+        """Like torch's, but the moments keep the types they are held in (torch casts floating state to the parameter's type), and a checkpoint
+        that is refused leaves the optimizer as it was."""
         if state_dict.get("state_bits", 32) != self.state_bits:
             raise ValueError("FusedAdamW: the checkpoint holds its moments in %d bits, the optimizer in %d"
                              % (state_dict.get("state_bits", 32), self.state_bits))
-        super().load_state_dict({k: v for k, v in state_dict.items() if k in ("state", "param_groups")})
-        self.seed = int(state_dict.get("seed", self.seed))
         params = [p for group in self.param_groups for p in group["params"]]
         places = [i for group in state_dict["param_groups"] for i in group["params"]]
+        made = {}                                            # (all of it is read before anything of the optimizer's changes)
         for p, place in zip(params, places):
             saved = state_dict["state"].get(place)
             if not saved:
                 continue
-            fresh = self._new_state(p)
+            fresh = made[p] = self._new_state(p)
             for key in self._keys():
-                if tuple(saved[key].shape) != tuple(fresh[key].shape):
+                if not isinstance(saved.get(key), torch.Tensor) or saved[key].shape != fresh[key].shape:
                     raise ValueError("FusedAdamW: %s of parameter %d has shape %s, expected %s"
-                                     % (key, place, tuple(saved[key].shape), tuple(fresh[key].shape)))
+                                     % (key, place, getattr(saved.get(key), "shape", None), tuple(fresh[key].shape)))
+                if fresh[key].dtype == torch.float8_e4m3fn and saved[key].dtype != torch.float8_e4m3fn:
+                    raise ValueError("FusedAdamW: %s of parameter %d is %s, expected e4m3 values" % (key, place, saved[key].dtype))
                 fresh[key].copy_(saved[key])
-            self.state[p] = dict(fresh, step=int(saved["step"]))
+            if "step" not in saved:
+                raise ValueError("FusedAdamW: parameter %d has no step count" % place)
+            fresh["step"] = int(saved["step"])
+        super().load_state_dict({"state": {}, "param_groups": state_dict["param_groups"]})
+        self.seed = int(state_dict.get("seed", self.seed))
+        self.state.update(made)
 
 
 OPTIMIZERS = {

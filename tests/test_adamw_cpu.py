@@ -106,3 +106,42 @@ def test_late_parameters_and_types_get_their_own_launches(launches, bits):
             p = next(p for p in params if p.numel() == row[6])
             assert row[:2 + len(KEYS[bits])].tolist() == [p.data_ptr(), p.grad.data_ptr()] + [opt.state[p][k].data_ptr() for k in KEYS[bits]]
     assert [opt.state[p]["step"] for p in params] == [2, 1, 2, 2, 2]
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("bits", [32, 8])
+def test_a_refused_checkpoint_changes_nothing(launches, bits, dtype):
+    """One moment of another shape or missing, an 8-bit one in another type, no step count, other groups: the optimizer stays as it was."""
+    params = _parameters(8, 300, dtype=dtype)
+    opt = FusedAdamW(params, state_bits=bits, seed=3)
+    opt.step()
+    before = [dict(opt.state[p]) for p in params]
+    good = {"state": {i: dict(opt.state[p]) for i, p in enumerate(params)}, "param_groups": [dict(opt.param_groups[0], params=[0, 1], lr=0.5)],
+            "state_bits": bits, "seed": 4}
+
+    def damaged(change):
+        out = dict(good, state={i: dict(st) for i, st in good["state"].items()}, param_groups=[dict(good["param_groups"][0])])
+        change(out)
+        return out
+
+    bad = [damaged(lambda c, key=key: c["state"][1].update({key: c["state"][1][key][:-1]})) for key in KEYS[bits]]
+    bad += [damaged(lambda c, key=key: c["state"][1].pop(key)) for key in KEYS[bits] + ["step"]]
+    bad += [damaged(lambda c: c["param_groups"][0].update(params=[0])), damaged(lambda c: c.update(state_bits=40 - bits)),
+            damaged(lambda c: c["param_groups"].append(dict(c["param_groups"][0])))]
+    if bits == 8:
+        bad.append(damaged(lambda c: c["state"][1].update(exp_avg=c["state"][1]["exp_avg"].float())))
+    for checkpoint in bad:
+        with pytest.raises(ValueError):
+            opt.load_state_dict(checkpoint)
+        assert opt.seed == 3 and opt.param_groups[0]["lr"] == 1e-3
+        for p, held in zip(params, before):
+            assert opt.state[p].keys() == held.keys() and all(opt.state[p][key] is held[key] for key in held)
+    opt.load_state_dict(good)
+    assert opt.seed == 4 and opt.param_groups[0]["lr"] == 0.5
+    for p, held in zip(params, before):
+        for key in KEYS[bits]:
+            assert opt.state[p][key] is not held[key] and opt.state[p][key].dtype == held[key].dtype
+            assert torch.equal(opt.state[p][key].view(torch.uint8), held[key].view(torch.uint8))
+        assert opt.state[p]["step"] == 1
+    opt.step()
+    assert opt.state[params[0]]["step"] == 2
