@@ -184,7 +184,16 @@ class FusedAdamW(Optimizer):
     def _held_dtype(self, key):
         return torch.float32 if self.state_bits == 32 or key.endswith("_scale") else torch.float8_e4m3fn
 
+    @staticmethod
+    def _known_options(group):
+        """A group's (or a checkpoint's) options that change torch's rule into one that this optimizer does not have."""
+        for option in ("amsgrad", "maximize"):
+            if group.get(option):
+                raise ValueError("FusedAdamW: %s is not supported" % option)
+
     def add_param_group(self, param_group):
+        if isinstance(param_group, dict):
+            self._known_options(param_group)
         super().add_param_group(param_group)
         params = self.param_groups[-1]["params"]
         if len(set(map(id, params))) != len(params):         # (one launch updates them side by side: twice would be a race)
@@ -305,6 +314,8 @@ class FusedAdamW(Optimizer):
         if state_dict.get("state_bits", 32) != self.state_bits:
             raise ValueError("FusedAdamW: the checkpoint holds its moments in %d bits, the optimizer in %d"
                              % (state_dict.get("state_bits", 32), self.state_bits))
+        for group in state_dict["param_groups"]:
+            self._known_options(group)
         params = [p for group in self.param_groups for p in group["params"]]
         places = [i for group in state_dict["param_groups"] for i in group["params"]]
         made = {}                                            # (all of it is read before anything of the optimizer's changes)

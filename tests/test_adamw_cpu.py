@@ -145,3 +145,22 @@ def test_a_refused_checkpoint_changes_nothing(launches, bits, dtype):
         assert opt.state[p]["step"] == 1
     opt.step()
     assert opt.state[params[0]]["step"] == 2
+
+
+@pytest.mark.parametrize("option", ["amsgrad", "maximize"])
+def test_options_that_change_the_rule_are_refused(option):
+    """torch.optim.AdamW's checkpoints carry them, and a group may: neither is dropped in silence.  Options that are off pass."""
+    p, q = _parameters(4, 4)
+    ref = torch.optim.AdamW([torch.nn.Parameter(torch.ones(4))], **{option: True})
+    opt = FusedAdamW([p], lr=0.25)
+    with pytest.raises(ValueError, match=option):
+        opt.load_state_dict(ref.state_dict())
+    assert opt.param_groups[0]["lr"] == 0.25
+    with pytest.raises(ValueError, match=option):
+        opt.add_param_group({"params": [q], option: True})
+    with pytest.raises(ValueError, match=option):
+        FusedAdamW([{"params": [p], option: True}])
+    assert len(opt.param_groups) == 1
+    opt.load_state_dict(torch.optim.AdamW([torch.nn.Parameter(torch.ones(4))], lr=0.125).state_dict())
+    opt.add_param_group({"params": [q], option: False})
+    assert opt.param_groups[0]["lr"] == 0.125 and len(opt.param_groups) == 2
