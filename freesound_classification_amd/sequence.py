@@ -8,6 +8,7 @@ scan states fp32; sums and states are fp32 inside, with one rounding at each out
 behind lengths[n] are never read (they may hold anything), give zeros and get zero gradients, and states pass them by unchanged.
 """
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import _lib
@@ -86,12 +87,17 @@ def _first(what, name, t, dims, shape):
 
 
 def _grad_needed(*tensors):
-    return torch.is_grad_enabled() and any([t is not None and t.requires_grad for t in tensors])
+    return (torch.is_grad_enabled() and any([t is not None and t.requires_grad for t in tensors])) or _has_tangent(tensors)
+
+
+def _has_tangent(tensors):
+    """Whether forward-mode derivatives arrive (they do not need requires_grad): autograd then refuses the function, which has none to pass on."""
+    return getattr(forward_ad, "_current_level", 0) >= 0 and any([t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors])
 
 
 def _one_frame(what, *tensors):
     if _grad_needed(*tensors):
-        _fail(what, "a single frame has no gradient: run it under torch.no_grad(), or the sequence operator for training")
+        _fail(what, "a single frame has no gradient and no forward derivative: run it under torch.no_grad(), or the sequence operator for training")
 
 
 def _once(backward):
@@ -184,7 +190,7 @@ def causal_conv_step(x, window, weight, bias=None, activation="silu"):
     n, d = x.shape
     taps = weight.shape[1]
     window = _state(what, "window", window, (n, taps - 1, d), x.dtype, device)
-    _one_frame(what, x, weight, bias)
+    _one_frame(what, x, weight, bias, window)
     y = x.new_empty((n, d))
     call("fsc_causal_conv_step",
          CausalConvArgs.packed(n, 1, d, taps, _DTYPES[x.dtype], int(activation is not None), x.data_ptr(), x.stride(0), 0, weight.data_ptr(),
@@ -298,7 +304,7 @@ def selective_scan_step(u, dt, a_log, b, c, state, d=None, z=None, dt_bias=None,
     what = "selective_scan_step"
     u, dt, a_log, b, c, d, z, dt_bias, device = _scan_inputs(what, 2, u, dt, a_log, b, c, d, z, dt_bias)
     state = _state(what, "state", state, (u.shape[0],) + tuple(a_log.shape), torch.float32, device)
-    _one_frame(what, u, dt, a_log, b, c, d, z, dt_bias)
+    _one_frame(what, u, dt, a_log, b, c, d, z, dt_bias, state)
     y = u.new_empty(u.shape)
     call("fsc_selective_scan_step", _scan_args(u, dt, a_log, b, c, d, z, dt_bias, int(bool(softplus)), None, None, y, state), stream_ptr())
     _moved_on(state)

@@ -2,9 +2,13 @@
 import ctypes as C
 
 import pytest
+import torch
+import torch.autograd.forward_ad as fwd
 
 import freesound_classification_amd as pkg
 from freesound_classification_amd import _lib
+from freesound_classification_amd import functional as F
+from freesound_classification_amd import sequence
 
 
 def _conv(**kw):
@@ -29,3 +33,47 @@ def test_sizes_of_empty_calls(length, empty):
     assert lib.fsc_causal_conv_bwd_workspace_bytes(C.byref(_conv(**kw))) == (0 if "channels" in empty else 4 * 5 * 8)
     assert lib.fsc_causal_conv_fwd(C.byref(_conv(**kw)), None) == 0
     assert lib.fsc_selective_scan_fwd(C.byref(_scan(**kw)), None) == 0
+
+
+@pytest.fixture
+def launches(monkeypatch):
+    """Host tensors stand for those of device 0; launches are noted instead of made."""
+    made = []
+    monkeypatch.setattr(torch.Tensor, "get_device", lambda t: 0)
+    monkeypatch.setattr(_lib, "_get_device", lambda: 0)
+    monkeypatch.setattr(sequence, "call", lambda name, *args: made.append(name))
+    monkeypatch.setattr(sequence, "stream_ptr", lambda: 0)
+    return made
+
+
+def _conv_call(p, step):
+    if step:
+        return F.causal_conv_step(p["x"][:, 0], p["window"], p["weight"], p["bias"])
+    return F.causal_conv(p["x"], p["weight"], p["bias"], initial=p["window"])
+
+
+def _scan_call(p, step):
+    if step:
+        return F.selective_scan_step(p["u"][:, 0], p["dt"][:, 0], p["a_log"], p["b"][:, 0], p["c"][:, 0], p["state"], d=p["d"], z=p["z"][:, 0], dt_bias=p["bias"])
+    return F.selective_scan(p["u"], p["dt"], p["a_log"], p["b"], p["c"], d=p["d"], z=p["z"], dt_bias=p["bias"], initial=p["state"])
+
+
+CALLS = {"conv": (_conv_call, dict(x=(2, 5, 8), weight=(8, 4), bias=(8,), window=(2, 3, 8))),
+         "scan": (_scan_call, dict(u=(2, 5, 8), dt=(2, 5, 8), z=(2, 5, 8), b=(2, 5, 16), c=(2, 5, 16), a_log=(8, 16), d=(8,), bias=(8,), state=(2, 8, 16)))}
+
+
+@pytest.mark.parametrize("grad_mode", [True, False])
+@pytest.mark.parametrize("step", [False, True])
+@pytest.mark.parametrize("operator, name", [(op, name) for op in CALLS for name in CALLS[op][1]])
+def test_forward_derivatives_are_refused(launches, operator, name, step, grad_mode):
+    """A dual number needs no requires_grad: its tangent must not get lost on the path that makes no autograd node."""
+    call, shapes = CALLS[operator]
+    p = {k: torch.ones(shape) for k, shape in shapes.items()}
+    with fwd.dual_level(), torch.set_grad_enabled(grad_mode):
+        call(p, step)
+        assert len(launches) == 1                        # (inside a level, but no tangent anywhere)
+        dual = dict(p, **{name: fwd.make_dual(p[name], torch.ones_like(p[name]))})
+        with pytest.raises((NotImplementedError, _lib.FscError) if not step else _lib.FscError, match="forward"):
+            call(dual, step)
+    call(p, step)
+    assert launches.count(launches[0]) == len(launches) <= (2 if step else 3)
