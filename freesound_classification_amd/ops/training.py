@@ -147,6 +147,8 @@ _dtype_of, _grad_of = operator.attrgetter("dtype"), operator.attrgetter("grad")
 _step_of = operator.itemgetter("step")
 _is_none = partial(operator.is_, None)
 _is_contiguous, _address, _numel, _device_number = torch.Tensor.is_contiguous, torch.Tensor.data_ptr, torch.Tensor.numel, torch.Tensor.get_device
+# (the kernels write through raw addresses; a graph that saved a weight in front of a step must not go on with the new one)
+_mark_changed = torch.autograd.graph.increment_version
 STATE_BLOCK = 256        # elements that share one scale of an 8-bit moment
 
 
@@ -300,6 +302,7 @@ class FusedAdamW(Optimizer):
         with F._stage("optimizer", sum(counts) * (3 * tensors[0].element_size() + 2 * held)):
             call("fsc_adamw_step", table.ctypes.data, n, _PARAM_DTYPES[dtype], self.state_bits, factors, dev, b1, b2,
                  float(group["eps"]), float(self.grad_scale), stream_ptr())
+        _mark_changed(itertools.chain(tensors, *moments))
         for st in states:
             st["step"] = step
 
@@ -460,6 +463,7 @@ class CapturedTrainingStep:
                                 "ONE `with torch.cuda.stream(s):` (not on the default stream; see the class docstring)")
         self.stream = stream
         self.model, self.opt = model, opt
+        self._changed = [t for p in trained for t in (p, *[opt.state[p][key] for key in opt._keys()])] if decoupled else []
         self.step_count = int(next(iter(opt.state.values()))["step"])
         self.signal = signal.clone()
         self.labels = labels.clone()
@@ -500,7 +504,7 @@ class CapturedTrainingStep:
         self.signal.copy_(signal, non_blocking=True)
         self.labels.copy_(labels, non_blocking=True)
         self.step_count += 1
-        # the replay rewrites parameters and BatchNorm buffers through raw pointers (no torch version bump): the caches of an
+        # the replay rewrites parameters and BatchNorm buffers through raw pointers (no torch version bump by itself): the caches of an
         # inference forward between replays (packed fragments, folded eval-mode BatchNorm) must not survive it
         from .. import functional
         functional.forget_packed_weights()
@@ -518,6 +522,7 @@ class CapturedTrainingStep:
                 call("fsc_fill", to, float(value), 1, stream_ptr())
                 to += 4
         self.graph.replay()
+        _mark_changed(self._changed)
         return self.outputs
 
     def sync_state(self):

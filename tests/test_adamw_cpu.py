@@ -164,3 +164,23 @@ def test_options_that_change_the_rule_are_refused(option):
     opt.load_state_dict(torch.optim.AdamW([torch.nn.Parameter(torch.ones(4))], lr=0.125).state_dict())
     opt.add_param_group({"params": [q], option: False})
     assert opt.param_groups[0]["lr"] == 0.125 and len(opt.param_groups) == 2
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_a_step_marks_what_it_changes(launches, bits):
+    """A graph that saved a weight (or a moment) must notice that a step has changed it; a parameter without a gradient is not touched."""
+    p, q = _parameters(5, 5)
+    q.grad = None
+    opt = FusedAdamW([p, q], state_bits=bits)
+    opt.step()
+    seen = [p._version, q._version] + [opt.state[p][key]._version for key in KEYS[bits]]
+    squares, others = p.square().sum(), q.square().sum()
+    scaled = None
+    if bits == 32:
+        scaled = (torch.ones(5, requires_grad=True) * opt.state[p]["exp_avg_sq"]).sum()
+    opt.step()
+    assert [p._version, q._version] + [opt.state[p][key]._version for key in KEYS[bits]] == [seen[0] + 1, seen[1]] + [v + 1 for v in seen[2:]]
+    for late in [squares] + ([scaled] if bits == 32 else []):
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            late.backward()
+    others.backward()

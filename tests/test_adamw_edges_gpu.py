@@ -1,0 +1,56 @@
+"""AdamW on the device: what a recorded training step leaves behind on the host."""
+import types
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+if not torch.cuda.is_available():
+    pytest.skip("needs an MI355X", allow_module_level=True)
+
+from freesound_classification_amd.ops.training import CapturedTrainingStep, FusedAdamW  # noqa: E402
+
+DEV = "cuda:0"
+
+
+class Tiny(torch.nn.Module):
+    """What CapturedTrainingStep needs of a model: here (x shape * weight + bias - y)^2, three parameters."""
+
+    def __init__(self, bits):
+        super().__init__()
+        gen = torch.Generator().manual_seed(7)
+        self.shape, self.weight, self.bias = (torch.nn.Parameter(torch.randn(300, generator=gen).to(DEV)) for _ in range(3))
+        self.optimizer = FusedAdamW([dict(params=[self.shape, self.weight]), dict(params=[self.bias], weight_decay=0.0)], lr=1e-2, state_bits=bits)
+        self._reducer = None
+        self.config = types.SimpleNamespace(train=types.SimpleNamespace(accumulation_steps=1), network=types.SimpleNamespace(output_dropout=0.0))
+
+    def training_step(self, x, y):
+        off = x * self.shape * self.weight + self.bias - y
+        loss = (off * off).mean()
+        loss.backward()
+        self.optimizer.step()
+        self.optimizer.zero_grad()
+        return off.detach(), (off * off).detach(), loss.detach()
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_replays_mark_what_they_change(bits):
+    """A graph of a weight kept over a replay must notice the change, as over an eager step."""
+    gen = torch.Generator(device=DEV).manual_seed(1)
+    x, y = (torch.randn(300, generator=gen, device=DEV) for _ in range(2))
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        model = Tiny(bits)
+        model.training_step(x, y)
+        step = CapturedTrainingStep(model, x, y)
+        for _ in range(2):
+            tensors = list(model.parameters()) + [v for p in model.parameters() for k, v in model.optimizer.state[p].items() if k != "step"]
+            seen = [t._version for t in tensors]
+            late = model.weight.square().sum()
+            step(x, y)
+            assert all(t._version > v for t, v in zip(tensors, seen))
+            with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+                late.backward()
+    torch.cuda.synchronize()
