@@ -193,6 +193,10 @@ class FusedAdamW(Optimizer):
             if group.get(option):
                 raise ValueError("FusedAdamW: %s is not supported" % option)
 
+    def __getstate__(self):
+        """(torch keeps defaults, state and groups alone; the width and the seed are part of what the state means)"""
+        return dict(super().__getstate__(), state_bits=self.state_bits, seed=self.seed, grad_scale=self.grad_scale, factors_dev=None)
+
     def add_param_group(self, param_group):
         if isinstance(param_group, dict):
             self._known_options(param_group)

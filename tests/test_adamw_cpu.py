@@ -1,6 +1,8 @@
 """AdamW's host side without a device: what a step looks at before it launches.  The launch itself is replaced by one that notes its table;
 tensors in host memory stand for those of device 0."""
+import copy
 import ctypes as C
+import io
 
 import numpy as np
 import pytest
@@ -184,3 +186,33 @@ def test_a_step_marks_what_it_changes(launches, bits):
         with pytest.raises(RuntimeError, match="modified by an inplace operation"):
             late.backward()
     others.backward()
+
+
+def _saved(opt):
+    """Through torch's pickle (the bare one cannot read e4m3 tensors back)."""
+    file = io.BytesIO()
+    torch.save(opt, file)
+    file.seek(0)
+    return torch.load(file, weights_only=False)
+
+
+@pytest.mark.parametrize("copied", [copy.deepcopy, _saved])
+@pytest.mark.parametrize("bits", [32, 8])
+def test_copies_of_the_optimizer(launches, bits, copied):
+    """A copy holds its moments in the same width, goes on with the same random numbers and the same scale, and has a step of its own."""
+    made, _ = launches
+    (p,) = _parameters(300)
+    opt = FusedAdamW([p], lr=0.5, state_bits=bits, seed=11)
+    opt.grad_scale = 0.25
+    opt.step()
+    opt.factors_dev = torch.zeros(4)                         # (of a recording that is being made: not the copy's)
+    twin = copied(opt)
+    assert (twin.state_bits, twin.seed, twin.grad_scale, twin.factors_dev) == (bits, 11, 0.25, None)
+    (q,) = twin.param_groups[0]["params"]
+    assert q is not p and twin.state[q]["step"] == 1 and twin.param_groups[0]["lr"] == 0.5
+    opt.factors_dev = None
+    for o, leaf in ((opt, p), (twin, q)):
+        leaf.grad = torch.ones_like(leaf)
+        o.step()
+    assert made[1][0][0, 7] == made[2][0][0, 7] == 11 and made[2][0][0, 0] == q.data_ptr() and made[1][1][-2] == made[2][1][-2] == 0.25
+    assert twin.state_dict()["state_bits"] == bits and twin.state_dict()["seed"] == 11
