@@ -95,7 +95,14 @@ class SsmHead(nn.Module):
             self.dt_proj.bias.copy_(rate + torch.log(-torch.expm1(-rate)))          # softplus(bias) = rate
         self.a_log = nn.Parameter(torch.log(torch.arange(1, states + 1, dtype=torch.float32)).repeat(inner, 1))
         self.d = nn.Parameter(torch.ones(inner))
+        self._mark()
+
+    def _mark(self):
         self.a_log.no_decay = self.d.no_decay = True
+
+    def __setstate__(self, state):                           # (copy.deepcopy and torch.load make parameters without the mark)
+        super().__setstate__(state)
+        self._mark()
 
     def forward(self, x):
         raise RuntimeError("the head runs inside functional.ssm_head")

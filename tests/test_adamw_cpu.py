@@ -9,6 +9,7 @@ import pytest
 import torch
 
 from freesound_classification_amd import _lib
+from freesound_classification_amd.networks.classifiers import SsmHead
 from freesound_classification_amd.ops import training
 from freesound_classification_amd.ops.training import FusedAdamW
 
@@ -216,3 +217,13 @@ def test_copies_of_the_optimizer(launches, bits, copied):
         o.step()
     assert made[1][0][0, 7] == made[2][0][0, 7] == 11 and made[2][0][0, 0] == q.data_ptr() and made[1][1][-2] == made[2][1][-2] == 0.25
     assert twin.state_dict()["state_bits"] == bits and twin.state_dict()["seed"] == 11
+
+
+@pytest.mark.parametrize("copied", [copy.deepcopy, _saved])
+def test_a_copied_head_keeps_its_time_constants_out_of_the_decay(copied):
+    model = torch.nn.Sequential(torch.nn.Linear(3, 4), SsmHead(6))
+    for module in (model, copied(model)):
+        opt = training.make_optimizer("adamw", module, 1e-3, 0.1)
+        rates = {id(p): group["weight_decay"] for group in opt.param_groups for p in group["params"]}
+        held = {name for name, p in module.named_parameters() if rates[id(p)] == 0.0}
+        assert held == {"0.bias", "1.norm.weight", "1.norm.bias", "1.in_proj.bias", "1.conv_bias", "1.dt_proj.bias", "1.a_log", "1.d"}
