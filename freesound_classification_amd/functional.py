@@ -15,7 +15,7 @@ import torch
 
 from . import _lib
 from ._lib import ConvDesc, call, ptr, stream_ptr
-from .sequence import causal_conv, causal_conv_step, selective_scan, selective_scan_step  # noqa: F401  (public here)
+from .sequence import causal_conv, causal_conv_step, once, selective_scan, selective_scan_step  # noqa: F401  (the operators are public here)
 
 BN_EPS = 1e-5
 LOG_EPS = 1e-4
@@ -1710,6 +1710,7 @@ class FrameNormFn(torch.autograd.Function):
         return xl
 
     @staticmethod
+    @once
     def backward(ctx, dxl):
         xm, mean, rstd, weight = ctx.saved_tensors
         n, c, h, w = ctx.shape
@@ -1737,6 +1738,7 @@ class FrameMeanFn(torch.autograd.Function):
         return out
 
     @staticmethod
+    @once
     def backward(ctx, dout):
         n, w, d = ctx.shape
         dy = _empty((n, w, d), dout)
@@ -1756,6 +1758,7 @@ class SplitColsFn(torch.autograd.Function):
         return tuple(pieces)
 
     @staticmethod
+    @once
     def backward(ctx, *grads):
         grads = [g.contiguous() for g in grads]
         full = _empty((grads[0].shape[0], sum(ctx.widths)), grads[0])
@@ -2449,6 +2452,7 @@ class LinearFn(torch.autograd.Function):
         return y
 
     @staticmethod
+    @once
     def backward(ctx, dy):
         x, weight = ctx.saved_tensors
         dy = dy.contiguous()

@@ -100,7 +100,7 @@ def _one_frame(what, *tensors):
         _fail(what, "a single frame has no gradient and no forward derivative: run it under torch.no_grad(), or the sequence operator for training")
 
 
-def _once(backward):
+def once(backward):
     """once_differentiable, whose own work (as much as a launch) is only done where a graph of the gradient is asked for."""
     guarded = once_differentiable(backward)
     return lambda ctx, *grads: (guarded if torch.is_grad_enabled() else backward)(ctx, *grads)
@@ -139,7 +139,7 @@ class CausalConvFn(torch.autograd.Function):
         return _conv_forward(x, weight, bias, initial, lengths, silu, want_final)
 
     @staticmethod
-    @_once
+    @once
     def backward(ctx, dy, dfinal):
         if dy is None and dfinal is None:
             return (None,) * 7
@@ -239,7 +239,7 @@ class SelectiveScanFn(torch.autograd.Function):
         return y, final
 
     @staticmethod
-    @_once
+    @once
     def backward(ctx, dy, dfinal):
         if dy is None and dfinal is None:
             return (None,) * 12

@@ -9,6 +9,7 @@ import freesound_classification_amd as pkg
 from freesound_classification_amd import _lib
 from freesound_classification_amd import functional as F
 from freesound_classification_amd import sequence
+from freesound_classification_amd.networks.classifiers import SsmHead
 
 
 def _conv(**kw):
@@ -77,3 +78,22 @@ def test_forward_derivatives_are_refused(launches, operator, name, step, grad_mo
             call(dual, step)
     call(p, step)
     assert launches.count(launches[0]) == len(launches) <= (2 if step else 3)
+
+
+def test_second_derivatives_of_the_head_are_refused(launches, monkeypatch):
+    """Every gradient of the head that is asked for with a graph says that it has none, rather than come back as a constant."""
+    monkeypatch.setattr(F, "call", lambda name, *args: launches.append(name))
+    monkeypatch.setattr(F, "ptr", lambda t: None)
+    monkeypatch.setattr(F, "stream_ptr", lambda: 0)
+    monkeypatch.setattr(F, "_need_cuda", lambda t, what: None)
+    head = SsmHead(6, inner=8)
+    out = torch.zeros(2, 6, 3, 5, requires_grad=True)
+    y = F.ssm_head(out, head)
+    leaves = [out] + list(head.parameters())
+    for graph in (False, True):
+        v = torch.ones_like(y).requires_grad_()
+        grads = torch.autograd.grad(y, leaves, v, create_graph=graph, retain_graph=True)
+        assert all(g.shape == leaf.shape and g.requires_grad == graph for g, leaf in zip(grads, leaves))
+    for g in grads:
+        with pytest.raises(RuntimeError, match="once_differentiable"):
+            g.sum().backward(retain_graph=True)
