@@ -307,9 +307,13 @@ __global__ __launch_bounds__(256) void first_block_1d_kernel(const float* __rest
 namespace fsc {
 
 hipError_t zero_async(void* p, size_t bytes, hipStream_t st) {
-    const long count = (long)(bytes / sizeof(float));
-    if (count > 0) hipLaunchKernelGGL(fill_kernel, dim3(grid_for(count)), dim3(256), 0, st, reinterpret_cast<float*>(p), 0.f, count);
-    return hipPeekAtLastError();
+    long count = (long)(bytes / sizeof(float));
+    if (count == 0) return hipSuccess;
+    float* to = reinterpret_cast<float*>(p);
+    float zero = 0.f;
+    void* args[] = {&to, &zero, &count};
+    // (this launch's own status: the last error may be an older one, of somebody else's call)
+    return hipLaunchKernel(reinterpret_cast<const void*>(fill_kernel), dim3(grid_for(count)), dim3(256), args, 0, st);
 }
 
 }  // namespace fsc
