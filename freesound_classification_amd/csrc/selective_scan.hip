@@ -167,10 +167,7 @@ __global__ __launch_bounds__(256) void scan_step_kernel(fsc_selective_scan_args 
         const float delta = a.softplus ? softplus2(dt[r]) : dt[r];
         float v = 0.f;
 #pragma unroll
-        for (int i = 0; i < NS; ++i) {
-            const float rate = __expf(al[r][i]);
-            al[r][i] = rate > FLT_MAX ? -FLT_MAX : -rate;
-        }
+        for (int i = 0; i < NS; ++i) al[r][i] = rate_of(al[r][i]);
 #pragma unroll
         for (int i = 0; i < NS; ++i) {
             h[r][i] = fmaf(__builtin_amdgcn_exp2f(delta * al[r][i]), h[r][i], delta * kLn2 * u[r] * b[i]);

@@ -36,3 +36,24 @@ def test_empty_axes(n, t, d):
     dirty((n, t, 16), (n, t, 16))
     for leaf, g in zip(leaves, torch.autograd.grad([y, final], leaves, [torch.ones_like(y), torch.ones_like(final)])):
         assert g.shape == leaf.shape and not g.any() and bool(torch.isfinite(g).all())
+
+
+def test_single_frames_take_the_rates_of_the_sequence():
+    """exp(a_log) of large a_log beside small time steps.  h' = exp(-r) h, r = dt exp(a_log) <= 3, in units u = 2^-24: exp(a_log) is off by 2 (one
+    unit in the last place), dt log2(e) by 2 (the constant and the product), their product by 1, each times r in the result; exp2 by 2 and the
+    last product by 1: (5 r + 3) u.  (An exponential by way of a rounded a_log log2(e) is off by a_log u, here up to 80, times r.)"""
+    n, d = 64, 48
+    gen = torch.Generator().manual_seed(41)
+    a_log = 40 + 40 * torch.rand(d, 1, generator=gen)
+    r = 0.1 + 2.9 * torch.rand(n, d, generator=gen).double()
+    dt = (r / torch.exp(a_log.double())[:, 0]).float()
+    h = torch.randn(n, d, 1, generator=gen)
+    r = dt.double() * torch.exp(a_log.double())[:, 0]
+    want = torch.exp(-r) * h[..., 0].double()
+    zeros, rows = torch.zeros(n, d, device=DEV), torch.zeros(n, 1, device=DEV)
+    state = h.to(DEV)
+    F.selective_scan_step(zeros, dt.to(DEV), a_log.to(DEV), rows, rows, state, softplus=False)
+    _, final = F.selective_scan(zeros[:, None], dt.to(DEV)[:, None], a_log.to(DEV), rows[:, None], rows[:, None], softplus=False, initial=h.to(DEV),
+                                return_final=True)
+    for got in (state, final):
+        assert bool(((got[..., 0].cpu().double() - want).abs() <= (5 * r + 3) * 2.0 ** -24 * want.abs()).all())
