@@ -136,6 +136,7 @@ struct ScanPlace {
     int zero_first, zero_end;    // its share of the tiles behind the sequence's end, which only get zeros
     bool whole;                  // every channel of the block exists and rows are read E channels at once
     bool real;                   // the scan lane has a channel
+    int row, col;                // its row of the LDS arrays [channel][frame] and first column of B's and C's: those of zeros where it has no state
     __device__ ScanPlace(const fsc_selective_scan_args& a, const ScanPlan& p, int& len) {
         // segments vary fastest but one: blocks of one sequence's segment, which read the same B and C, follow one another
         const int per = p.blocks * p.segments;
@@ -161,7 +162,14 @@ struct ScanPlace {
         sg = threadIdx.x % L;
         real = channel_of(ch, E) < have;
         channel = c0 + (real ? channel_of(ch, E) : 0);
+        // (a lane without states must not meet what is not finite in its neighbours': it would carry NaN into the sums over states and channels)
+        const bool on = real && sg * NS < a.states;
+        row = on ? ch : CB;
+        col = on ? sg * NS : SP;
     }
+    // whether the lane's i-th state exists; PARTIAL: the last lane with states has fewer than NS, the others are kept at 0 element by element
+    template <bool PARTIAL>
+    __device__ bool has(int i, int states) const { return !PARTIAL || sg * NS + i < states; }
     // LDS row of the elementwise thread's i-th channel
     __device__ int lds_row(int i) const { return (threadIdx.x & 15) + 16 * i; }
     // element (row, state) of a B / C tile that this thread stages as its j-th
@@ -234,12 +242,22 @@ struct ScanRows {
         for (int j = 0; j < R; ++j)
             v[j].wide(reinterpret_cast<const T*>(at + (row(w, j) <= last ? off[j] : (uint32_t)last * (uint32_t)time + col[j])));
     }
-    __device__ __forceinline__ void stage(const Place& w, float (*to)[Place::SP], int tile, int len, int states, float unit) const {
+    __device__ __forceinline__ void stage(const Place& w, float (*to)[Place::SP + NS], int tile, int len, int states, float unit) const {
 #pragma unroll
         for (int j = 0; j < R; ++j)
             if (w.bc_mine(j)) to[w.bc_row(j)][w.bc_state(j)] = tile * kTile + w.bc_row(j) < len && w.bc_state(j) < states ? v[j][0] * unit : 0.f;
     }
 };
+
+// The LDS rows and columns of zeros, for lanes without states; visible behind the next barrier.
+template <int ROWS>
+__device__ __forceinline__ void scan_zero_row(float (&to)[ROWS][kPad]) {
+    if (threadIdx.x < kPad) to[ROWS - 1][threadIdx.x] = 0.f;
+}
+template <int NS, int COLUMNS>
+__device__ __forceinline__ void scan_zero_columns(float (&to)[kTile][COLUMNS]) {
+    if (threadIdx.x < kTile * NS) to[threadIdx.x / NS][COLUMNS - NS + threadIdx.x % NS] = 0.f;
+}
 
 // An output row (batch, length, channels) of frame te of a tile, first channel ce of the block.
 template <typename T, int L, int NS>
@@ -306,6 +324,13 @@ void with_scan_shape(const ScanPlan& p, Fn fn) {
     else if (p.per_lane == 4) fn(std::integral_constant<int, 4>(), std::integral_constant<int, 4>());
     else if (p.per_lane == 2) fn(std::integral_constant<int, 4>(), std::integral_constant<int, 2>());
     else fn(std::integral_constant<int, 4>(), std::integral_constant<int, 1>());
+}
+
+// fn(flag) with the flag as a type
+template <typename Fn>
+void with_flag(bool flag, Fn fn) {
+    if (flag) fn(std::true_type());
+    else fn(std::false_type());
 }
 
 }  // namespace fsc

@@ -28,15 +28,19 @@ struct Carve {
     }
 };
 
-// A segment's gradient of the state in front of it, from zero behind it: G as in the main pass, nothing else.
-template <typename T, int L, int NS>
+// A segment's gradient of the state in front of it, from zero behind it: G as in the main pass, nothing else.  (PARTIAL: as in the forward; 8 x 2048 x
+// 1024, a training step: 22 states 641 us, 24 states 590.)
+template <typename T, int L, int NS, bool PARTIAL>
 __global__ __launch_bounds__(256) void scan_bwd_ends_kernel(fsc_selective_scan_args a, ScanPlan p, float* ends, float* end_deltas) {
     using Place = ScanPlace<L, NS>;
     constexpr int CB = Place::CB, E = Place::E, SP = Place::SP;
-    __shared__ __align__(16) float s_delta[CB][kPad], s_dyy[CB][kPad], s_c[kTile][SP];
+    __shared__ __align__(16) float s_delta[CB + 1][kPad], s_dyy[CB + 1][kPad], s_c[kTile][SP + NS];
     int len;
     const Place w(a, p, len);
     if (w.segment == 0) return;
+    scan_zero_row(s_delta);
+    scan_zero_row(s_dyy);
+    scan_zero_columns<NS>(s_c);
     float rate[NS], e[NS] = {}, sum = 0.f;
     scan_rates(a, w, rate);
     float bias[E];
@@ -76,14 +80,17 @@ __global__ __launch_bounds__(256) void scan_bwd_ends_kernel(fsc_selective_scan_a
 #pragma unroll
         for (int q = kTile / 4 - 1; q >= 0; --q) {
             float dl[4], dyy[4];
-            load_row<4>(&s_delta[w.ch][4 * q], true, 4, dl);
-            load_row<4>(&s_dyy[w.ch][4 * q], true, 4, dyy);
+            load_row<4>(&s_delta[w.row][4 * q], true, 4, dl);
+            load_row<4>(&s_dyy[w.row][4 * q], true, 4, dyy);
 #pragma unroll
             for (int j = 3; j >= 0; --j) {
                 float cc[NS];
-                load_row<NS>(&s_c[4 * q + j][w.sg * NS], true, NS, cc);
+                load_row<NS>(&s_c[4 * q + j][w.col], true, NS, cc);
 #pragma unroll
-                for (int i = 0; i < NS; ++i) e[i] = __builtin_amdgcn_exp2f(dl[j] * rate[i]) * fmaf(cc[i], dyy[j], e[i]);
+                for (int i = 0; i < NS; ++i) {
+                    e[i] = __builtin_amdgcn_exp2f(dl[j] * rate[i]) * fmaf(cc[i], dyy[j], e[i]);
+                    e[i] = w.template has<PARTIAL>(i, a.states) ? e[i] : 0.f;
+                }
                 sum += dl[j];
             }
         }
@@ -122,18 +129,23 @@ __device__ __forceinline__ void channel_sums(float (&v)[2 * NS]) {
     }
 }
 
-template <typename T, int L, int NS>
+template <typename T, int L, int NS, bool PARTIAL>
 __global__ __launch_bounds__(256, 2) void scan_bwd_kernel(fsc_selective_scan_args a, ScanPlan p, Carve at) {
     using Place = ScanPlace<L, NS>;
     constexpr int CB = Place::CB, E = Place::E, SP = Place::SP;
-    __shared__ __align__(16) float s_delta[CB][kPad], s_du[CB][kPad], s_dyy[CB][kPad], s_yh[CB][kPad], s_gb[CB][kPad], s_ga[CB][kPad];
+    __shared__ __align__(16) float s_delta[CB + 1][kPad], s_du[CB + 1][kPad], s_dyy[CB + 1][kPad], s_yh[CB][kPad], s_gb[CB][kPad], s_ga[CB][kPad];
     __shared__ __align__(16) float s_sig[256][E], s_gz[256][E];       // a thread's own, out of its registers while it scans
-    __shared__ __align__(16) float s_b[kTile][SP], s_c[kTile][SP];
+    __shared__ __align__(16) float s_b[kTile][SP + NS], s_c[kTile][SP + NS];
     __shared__ __align__(16) float s_red[kTile][4][2][SP];
     float* ws = reinterpret_cast<float*>(a.workspace);
     int len;
     const Place w(a, p, len);
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    scan_zero_row(s_delta);
+    scan_zero_row(s_du);
+    scan_zero_row(s_dyy);
+    scan_zero_columns<NS>(s_b);
+    scan_zero_columns<NS>(s_c);
 
     float rate[NS], e[NS], da[NS] = {};              // e: exp(delta_{t+1} A) G_{t+1}, what reaches h_t from behind
     scan_rates(a, w, rate);
@@ -144,7 +156,7 @@ __global__ __launch_bounds__(256, 2) void scan_bwd_kernel(fsc_selective_scan_arg
         float more[NS];
         load_row<NS>(ws + at.ends + w.end(p, q), true, NS, more);
 #pragma unroll
-        for (int i = 0; i < NS; ++i) e[i] = fmaf(__builtin_amdgcn_exp2f(rate[i] * ds), e[i], more[i]);
+        for (int i = 0; i < NS; ++i) e[i] = w.real && w.sg * NS + i < a.states ? fmaf(__builtin_amdgcn_exp2f(rate[i] * ds), e[i], more[i]) : 0.f;
     }
     float bias[E], skip[E], dskip[E] = {}, dbias[E] = {};
     scan_param(w, a.dt_bias, bias);
@@ -179,7 +191,7 @@ __global__ __launch_bounds__(256, 2) void scan_bwd_kernel(fsc_selective_scan_arg
     pin_all(bias);
     pin_all(skip);
     for (int tile = w.work_end - 1; tile >= w.first; --tile) {
-        const int t = tile * kTile + w.te;
+        const int t = tile * kTile + w.te, count = len - tile * kTile;
         const Raw<T, E> u_now = u_next;
         float raw[E], delta[E], dyy[E], sig[E], gz[E], h[NS], hp[kTile][NS], ex[kTile][NS];
         time_steps(dt_next, bias, a.softplus, t < len, raw, delta);
@@ -219,18 +231,19 @@ __global__ __launch_bounds__(256, 2) void scan_bwd_kernel(fsc_selective_scan_arg
 #pragma unroll
         for (int q = 0; q < kTile / 4; ++q) {
             float dl[4], du[4], y[4];
-            load_row<4>(&s_delta[w.ch][4 * q], true, 4, dl);
-            load_row<4>(&s_du[w.ch][4 * q], true, 4, du);
+            load_row<4>(&s_delta[w.row][4 * q], true, 4, dl);
+            load_row<4>(&s_du[w.row][4 * q], true, 4, du);
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
                 float b[NS], cc[NS], v = 0.f;
-                load_row<NS>(&s_b[4 * q + j][w.sg * NS], true, NS, b);
-                load_row<NS>(&s_c[4 * q + j][w.sg * NS], true, NS, cc);
+                load_row<NS>(&s_b[4 * q + j][w.col], true, NS, b);
+                load_row<NS>(&s_c[4 * q + j][w.col], true, NS, cc);
 #pragma unroll
                 for (int i = 0; i < NS; ++i) {
-                    ex[4 * q + j][i] = __builtin_amdgcn_exp2f(dl[j] * rate[i]);
+                    const bool has = w.template has<PARTIAL>(i, a.states);
+                    ex[4 * q + j][i] = has ? __builtin_amdgcn_exp2f(dl[j] * rate[i]) : 0.f;
                     hp[4 * q + j][i] = h[i];
-                    h[i] = fmaf(ex[4 * q + j][i], h[i], du[j] * b[i]);
+                    h[i] = has ? fmaf(ex[4 * q + j][i], h[i], du[j] * b[i]) : 0.f;
                     v = fmaf(cc[i], h[i], v);
                 }
                 y[j] = group_sum<L>(v);
@@ -240,19 +253,20 @@ __global__ __launch_bounds__(256, 2) void scan_bwd_kernel(fsc_selective_scan_arg
         }
 #pragma unroll
         for (int q = kTile / 4 - 1; q >= 0; --q) {
-            float dl[4], du[4], dyy4[4], gb4[4], ga4[4];
-            load_row<4>(&s_delta[w.ch][4 * q], true, 4, dl);
-            load_row<4>(&s_du[w.ch][4 * q], true, 4, du);
-            load_row<4>(&s_dyy[w.ch][4 * q], true, 4, dyy4);
+            float dl[4], du[4], dyy4[4], gb4[4] = {}, ga4[4] = {};
+            load_row<4>(&s_delta[w.row][4 * q], true, 4, dl);
+            load_row<4>(&s_du[w.row][4 * q], true, 4, du);
+            load_row<4>(&s_dyy[w.row][4 * q], true, 4, dyy4);
 #pragma unroll
             for (int j = 3; j >= 0; --j) {
                 const int k = 4 * q + j;
+                if (k >= count) continue;             // (a frame behind the end: its delta of 0 would make NaN of an infinite state)
                 float b[NS], cc[NS], v[2 * NS], gb = 0.f, ga = 0.f;
-                load_row<NS>(&s_b[k][w.sg * NS], true, NS, b);
-                load_row<NS>(&s_c[k][w.sg * NS], true, NS, cc);
+                load_row<NS>(&s_b[k][w.col], true, NS, b);
+                load_row<NS>(&s_c[k][w.col], true, NS, cc);
 #pragma unroll
                 for (int i = 0; i < NS; ++i) {
-                    const float g = fmaf(cc[i], dyy4[j], e[i]);
+                    const float g = w.template has<PARTIAL>(i, a.states) ? fmaf(cc[i], dyy4[j], e[i]) : 0.f;
                     v[i] = g * du[j];
                     v[NS + i] = h[i] * dyy4[j];
                     gb = fmaf(g, b[i], gb);
@@ -288,7 +302,7 @@ __global__ __launch_bounds__(256, 2) void scan_bwd_kernel(fsc_selective_scan_arg
         for (int j = threadIdx.x; j < kTile * 2 * SP; j += 256) {
             const int k = j / (2 * SP), rest = j % (2 * SP);
             const float* r = &s_red[k][0][0][rest];
-            ws[at.rows + w.rows(p, tile) + j] = (r[0] + r[2 * SP]) + (r[4 * SP] + r[6 * SP]);
+            ws[at.rows + w.rows(p, tile) + j] = k < count ? (r[0] + r[2 * SP]) + (r[4 * SP] + r[6 * SP]) : 0.f;
         }
         if (t < a.length) {
             float du_out[E], ddt_out[E], dz_out[E];
@@ -431,10 +445,13 @@ int fsc_selective_scan_bwd(const fsc_selective_scan_args* args_host, fsc_stream_
         if (a.batch > 0 && a.channels > 0)               // (without channels db and dc are still there: sums over nothing)
             with_scan_shape(p, [&](auto lanes, auto per) {
                 constexpr int L = decltype(lanes)::value, NS = decltype(per)::value;
-                if (p.segments > 1)
-                    hipLaunchKernelGGL((scan_bwd_ends_kernel<T, L, NS>), grid, dim3(256), 0, as_stream(stream), a, p, ws + at.ends,
-                                       ws + at.end_deltas);
-                hipLaunchKernelGGL((scan_bwd_kernel<T, L, NS>), grid, dim3(256), 0, as_stream(stream), a, p, at);
+                with_flag(a.states % NS != 0, [&](auto partial) {
+                    constexpr bool PARTIAL = decltype(partial)::value;
+                    if (p.segments > 1)
+                        hipLaunchKernelGGL((scan_bwd_ends_kernel<T, L, NS, PARTIAL>), grid, dim3(256), 0, as_stream(stream), a, p, ws + at.ends,
+                                           ws + at.end_deltas);
+                    hipLaunchKernelGGL((scan_bwd_kernel<T, L, NS, PARTIAL>), grid, dim3(256), 0, as_stream(stream), a, p, at);
+                });
             });
         hipLaunchKernelGGL((scan_bwd_finish_kernel<T>), dim3((unsigned)(rows + columns)), dim3(256), 0, as_stream(stream), a, p, at, rows);
     };

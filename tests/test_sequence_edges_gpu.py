@@ -8,6 +8,7 @@ if not torch.cuda.is_available():
     pytest.skip("needs an MI355X", allow_module_level=True)
 
 from freesound_classification_amd import functional as F  # noqa: E402
+from oracle import sequence as oseq  # noqa: E402
 
 DEV = "cuda:0"
 
@@ -57,3 +58,45 @@ def test_single_frames_take_the_rates_of_the_sequence():
                                 return_final=True)
     for got in (state, final):
         assert bool(((got[..., 0].cpu().double() - want).abs() <= (5 * r + 3) * 2.0 ** -24 * want.abs()).all())
+
+
+def same_kinds(got, want, frames, what):
+    """Infinities and NaN where the definition has them, of the same sign; the others to 10 (4 T + 32) u of their 2-norm, as in the sequence tests."""
+    got, want = got.detach().cpu().double(), want.detach()
+    assert got.shape == want.shape, what
+    for kind in (torch.isnan, torch.isposinf, torch.isneginf):
+        assert torch.equal(kind(got), kind(want)), (what, kind.__name__, int((kind(got) != kind(want)).sum()))
+    fine = torch.isfinite(want)
+    off = float((got[fine] - want[fine]).norm())
+    assert off <= 10 * (4 * frames + 32) * 2.0 ** -24 * float(want[fine].norm()) + 1e-30, (what, off)
+
+
+@pytest.mark.parametrize("where", ["u", "dt"])
+@pytest.mark.parametrize("n, t, d, s, g, at, length", [
+    (1, 40, 64, 16, 1, 9, None), (1, 40, 70, 5, 1, 9, None), (2, 40, 70, 16, 2, 20, None), (1, 21, 12, 3, 1, 0, None), (1, 30, 33, 24, 1, 17, None),
+    (1, 20, 20, 33, 1, 3, None), (1, 20, 5, 1, 1, 3, None), (1, 400, 40, 5, 1, 333, None), (1, 400, 70, 17, 2, 20, None), (2, 40, 70, 5, 1, 32, 33),
+    (2, 40, 64, 16, 1, 20, 21), (1, 300, 24, 12, 1, 199, 200)])
+def test_infinities_stay_infinities(n, t, d, s, g, at, length, where):
+    """One infinite value in the last channel at frame `at`, everything else positive, so that no infinities of two signs meet: outputs and
+    gradients are infinite where the recurrence's are, whatever states and channels the lanes are padded with, and the frames behind a
+    sequence's end get their zeros."""
+    gen = torch.Generator().manual_seed(d + s + at)
+    pos = lambda *shape: 0.2 + torch.rand(*shape, generator=gen)  # noqa: E731
+    p = dict(u=pos(n, t, d), dt=pos(n, t, d) - 1.0, a_log=pos(d, s), b=pos(n, t, g, s), c=pos(n, t, g, s), d=pos(d), z=pos(n, t, d), dt_bias=pos(d) - 1.0,
+             initial=pos(n, d, s))
+    p[where][0, at, d - 1] = float("inf")
+    lengths = None if length is None else [length] + [t] * (n - 1)
+    cot = pos(n, t, d), pos(n, d, s)
+    if length is not None:
+        cot[0][0, length:] = float("nan")                    # (never read)
+    dev = {k: v.to(DEV).requires_grad_() for k, v in p.items()}
+    ref = {k: v.double().requires_grad_() for k, v in p.items()}
+    got = F.selective_scan(dev["u"], dev["dt"], dev["a_log"], dev["b"], dev["c"], d=dev["d"], z=dev["z"], dt_bias=dev["dt_bias"], initial=dev["initial"],
+                           lengths=None if lengths is None else torch.tensor(lengths, dtype=torch.int32, device=DEV), return_final=True)
+    want = oseq.selective_scan(ref["u"], ref["dt"], ref["a_log"], ref["b"], ref["c"], ref["d"], ref["z"], ref["dt_bias"], True, lengths, ref["initial"])
+    for name, a, b in zip(("y", "final"), got, want):
+        same_kinds(a, b, t, name)
+    grads = torch.autograd.grad(got, list(dev.values()), [v.to(DEV) for v in cot])
+    clean = [torch.nan_to_num(v.double(), nan=0.0) for v in cot]
+    for name, a, b in zip(p, grads, torch.autograd.grad(want, list(ref.values()), clean)):
+        same_kinds(a, b, t, "d" + name)
