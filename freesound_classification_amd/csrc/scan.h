@@ -288,6 +288,13 @@ __device__ __forceinline__ void scan_rates(const fsc_selective_scan_args& a, con
     for (int i = 0; i < NS; ++i) rate[i] = w.real && w.sg * NS + i < a.states ? rate_of(rate[i]) : 0.f;
 }
 
+// A state behind a segment: what was in front of it times the segment's decay, and the segment's end from zero.  An infinity outlasts every decay, also
+// one that is 0 in fp32 (frame by frame it meets factors above 0), unless a time step itself was infinite.
+__device__ __forceinline__ float scan_join(float h, float rate, float sum_delta, float end) {
+    const float decay = __builtin_amdgcn_exp2f(rate * sum_delta);
+    return fabsf(h) == INFINITY && sum_delta < INFINITY ? h + end : fmaf(decay, h, end);
+}
+
 // The lane's states of a (batch, channels, states) tensor, zeros without one.
 template <int L, int NS>
 __device__ __forceinline__ void scan_state(const fsc_selective_scan_args& a, const ScanPlace<L, NS>& w, const float* from, float (&h)[NS]) {

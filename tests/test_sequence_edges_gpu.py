@@ -71,20 +71,20 @@ def same_kinds(got, want, frames, what):
     assert off <= 10 * (4 * frames + 32) * 2.0 ** -24 * float(want[fine].norm()) + 1e-30, (what, off)
 
 
-@pytest.mark.parametrize("where", ["u", "dt"])
+@pytest.mark.parametrize("where", ["u", "dt", "b", "c"])
 @pytest.mark.parametrize("n, t, d, s, g, at, length", [
     (1, 40, 64, 16, 1, 9, None), (1, 40, 70, 5, 1, 9, None), (2, 40, 70, 16, 2, 20, None), (1, 21, 12, 3, 1, 0, None), (1, 30, 33, 24, 1, 17, None),
     (1, 20, 20, 33, 1, 3, None), (1, 20, 5, 1, 1, 3, None), (1, 400, 40, 5, 1, 333, None), (1, 400, 70, 17, 2, 20, None), (2, 40, 70, 5, 1, 32, 33),
     (2, 40, 64, 16, 1, 20, 21), (1, 300, 24, 12, 1, 199, 200)])
 def test_infinities_stay_infinities(n, t, d, s, g, at, length, where):
-    """One infinite value in the last channel at frame `at`, everything else positive, so that no infinities of two signs meet: outputs and
+    """One infinite value in the last channel (the last state of the last group) at frame `at`, everything else positive, so that no infinities of two signs meet: outputs and
     gradients are infinite where the recurrence's are, whatever states and channels the lanes are padded with, and the frames behind a
     sequence's end get their zeros."""
     gen = torch.Generator().manual_seed(d + s + at)
     pos = lambda *shape: 0.2 + torch.rand(*shape, generator=gen)  # noqa: E731
     p = dict(u=pos(n, t, d), dt=pos(n, t, d) - 1.0, a_log=pos(d, s), b=pos(n, t, g, s), c=pos(n, t, g, s), d=pos(d), z=pos(n, t, d), dt_bias=pos(d) - 1.0,
              initial=pos(n, d, s))
-    p[where][0, at, d - 1] = float("inf")
+    p[where][0, at].view(-1)[-1] = float("inf")
     lengths = None if length is None else [length] + [t] * (n - 1)
     cot = pos(n, t, d), pos(n, d, s)
     if length is not None:
