@@ -191,6 +191,8 @@ __global__ __launch_bounds__(kThreads) void conv_bwd_kernel(fsc_causal_conv_args
         const int n = (int)(row / p.strips), s = (int)(row % p.strips);
         const int len = frames_of(a, n);
         const int t0 = s * p.strip, t1 = t0 + p.strip < a.length ? t0 + p.strip : a.length;
+        // (frames past the strip are summed by the next one, and none behind the end: 0 times a frame that is not finite is not 0)
+        const int counted = a.dy == nullptr ? t0 : t1 < len ? t1 : len;
         float x[K - 1 + U][V], dp[K - 1 + U][V];
         window<T, K, V>(a, n, c, t0, len, wide, have, x);
 #pragma unroll
@@ -215,7 +217,7 @@ __global__ __launch_bounds__(kThreads) void conv_bwd_kernel(fsc_causal_conv_args
             if (t + U < t1 + K - 1) ahead(t + U);
 #pragma unroll
             for (int j = 0; j < U; ++j) {
-                const bool there = t + j < len && a.dy != nullptr, sum = t + j < t1;      // (frames past the strip are summed by the next one)
+                const bool there = t + j < len && a.dy != nullptr;
                 float grad[V];
 #pragma unroll
                 for (int i = 0; i < V; ++i) grad[i] = dy[j][i];
@@ -234,13 +236,17 @@ __global__ __launch_bounds__(kThreads) void conv_bwd_kernel(fsc_causal_conv_args
                     fsc::pin(grad[i]);               // (computed by every lane: a branch around it would cost more)
                     grad[i] = there ? grad[i] : 0.f;
                     dp[K - 1 + j][i] = grad[i];
-                    grad[i] = sum ? grad[i] : 0.f;
-                    db[i] += grad[i];
-                    fsc::pin(db[i]);
+                }
+                if (t + j < counted) {
 #pragma unroll
-                    for (int k = 0; k < K; ++k) {
-                        dw[k][i] = fmaf(grad[i], x[j + k][i], dw[k][i]);
-                        fsc::pin(dw[k][i]);
+                    for (int i = 0; i < V; ++i) {
+                        db[i] += grad[i];
+                        fsc::pin(db[i]);
+#pragma unroll
+                        for (int k = 0; k < K; ++k) {
+                            dw[k][i] = fmaf(grad[i], x[j + k][i], dw[k][i]);
+                            fsc::pin(dw[k][i]);
+                        }
                     }
                 }
                 const int at = t + j - (K - 1);

@@ -100,3 +100,30 @@ def test_infinities_stay_infinities(n, t, d, s, g, at, length, where):
     clean = [torch.nan_to_num(v.double(), nan=0.0) for v in cot]
     for name, a, b in zip(p, grads, torch.autograd.grad(want, list(ref.values()), clean)):
         same_kinds(a, b, t, "d" + name)
+
+
+@pytest.mark.parametrize("value", [float("inf"), float("nan")])
+@pytest.mark.parametrize("n, t, d, k, at, length, initial", [
+    (1, 24, 8, 4, 23, None, True), (1, 24, 8, 4, 8, None, False), (2, 100, 12, 8, 62, 64, True), (1, 70, 5, 3, 69, None, False), (1, 9, 8, 2, 0, 1, True),
+    (2, 40, 64, 4, 7, None, True), (1, 33, 7, 5, 30, 32, False), (1, 3000, 8, 4, 1500, None, True)])
+def test_what_is_not_finite_stays_with_its_taps(n, t, d, k, at, length, initial, value):
+    """One value of x that is not finite, no activation: each tap's gradient holds it where the tap meets it in a frame that exists, the last taps of a
+    sequence's last frames do not; the strips that time is cut into and the frames behind the end do not spread it."""
+    gen = torch.Generator().manual_seed(t + k)
+    pos = lambda *shape: 0.2 + torch.rand(*shape, generator=gen)  # noqa: E731
+    p = dict(x=pos(n, t, d), weight=pos(d, k), bias=pos(d))
+    if initial:
+        p["initial"] = pos(n, k - 1, d)
+    p["x"][0, at, d - 1] = value
+    lengths = None if length is None else [length] + [t] * (n - 1)
+    cot = pos(n, t, d), pos(n, k - 1, d)
+    dev = {key: v.to(DEV).requires_grad_() for key, v in p.items()}
+    ref = {key: v.double().requires_grad_() for key, v in p.items()}
+    got = F.causal_conv(dev["x"], dev["weight"], dev["bias"], activation=None, initial=dev.get("initial"),
+                        lengths=None if lengths is None else torch.tensor(lengths, dtype=torch.int32, device=DEV), return_final=True)
+    want = oseq.causal_conv(ref["x"], ref["weight"], ref["bias"], False, lengths, ref.get("initial"))
+    for name, a, b in zip(("y", "final"), got, want):
+        same_kinds(a, b, 1, name)
+    grads = torch.autograd.grad(got, list(dev.values()), [v.to(DEV) for v in cot])
+    for name, a, b in zip(p, grads, torch.autograd.grad(want, list(ref.values()), [v.double() for v in cot])):
+        same_kinds(a, b, 1 if name != "weight" and name != "bias" else n * t, "d" + name)
