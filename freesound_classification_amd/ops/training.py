@@ -467,8 +467,7 @@ class CapturedTrainingStep:
                                 "ONE `with torch.cuda.stream(s):` (not on the default stream; see the class docstring)")
         self.stream = stream
         self.model, self.opt = model, opt
-        self._changed = [t for p in trained for t in (p, *[opt.state[p][key] for key in opt._keys()])] if decoupled else []
-        self.step_count = int(next(iter(opt.state.values()))["step"])
+        self.step_count = int(opt.state[trained[0]]["step"]) if trained else 0
         self.signal = signal.clone()
         self.labels = labels.clone()
         per_group = 4 if decoupled else 2
@@ -487,9 +486,10 @@ class CapturedTrainingStep:
                     self.outputs = model.training_step(self.signal, self.labels)
         finally:
             opt.factors_dev = None
-        # the recording ran the step's Python (not its kernels): undo the one host-side effect, the step counters
-        for st in opt.state.values():
-            st["step"] = self.step_count
+            # the recording ran the step's Python (not its kernels): undo the one host-side effect, the step counters of what got a gradient
+            self._trained = [p for p in trained if int(opt.state[p]["step"]) != self.step_count]
+            self.sync_state()
+        self._changed = [t for p in self._trained for t in (p, *[opt.state[p][key] for key in opt._keys()])] if decoupled else []
         stale = [w for w in caught if "AccumulateGrad" in str(w.message)]
         for w in caught:
             if w not in stale:
@@ -512,8 +512,7 @@ class CapturedTrainingStep:
         # inference forward between replays (packed fragments, folded eval-mode BatchNorm) must not survive it
         from .. import functional
         functional.forget_packed_weights()
-        for st in self.opt.state.values():                # (a checkpoint saved mid-run resumes with the right bias correction)
-            st["step"] = self.step_count
+        self.sync_state()                                 # (a checkpoint saved mid-run resumes with the right bias correction)
         to = self.factors.data_ptr()
         for group in self.opt.param_groups:
             b1, b2 = group["betas"]
@@ -530,6 +529,7 @@ class CapturedTrainingStep:
         return self.outputs
 
     def sync_state(self):
-        """Write the step count back into the optimizer's state (state_dict compatibility) -- call before saving."""
-        for st in self.opt.state.values():
-            st["step"] = self.step_count
+        """Write the step count back into the optimizer's state (state_dict compatibility) -- call before saving.  (Parameters that the recorded step
+        does not change may have a state of earlier steps: it stays as it is.)"""
+        for p in self._trained:
+            self.opt.state[p]["step"] = self.step_count

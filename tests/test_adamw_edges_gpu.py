@@ -15,7 +15,9 @@ DEV = "cuda:0"
 
 
 class Tiny(torch.nn.Module):
-    """What CapturedTrainingStep needs of a model: here (x shape * weight + bias - y)^2, three parameters."""
+    """What CapturedTrainingStep needs of a model: here (x shape * weight + bias - y)^2, three parameters (`spare`: the shape is not used)."""
+
+    spare = False
 
     def __init__(self, bits):
         super().__init__()
@@ -26,7 +28,7 @@ class Tiny(torch.nn.Module):
         self.config = types.SimpleNamespace(train=types.SimpleNamespace(accumulation_steps=1), network=types.SimpleNamespace(output_dropout=0.0))
 
     def training_step(self, x, y):
-        off = x * self.shape * self.weight + self.bias - y
+        off = (x if self.spare else x * self.shape) * self.weight + self.bias - y
         loss = (off * off).mean()
         loss.backward()
         self.optimizer.step()
@@ -53,4 +55,31 @@ def test_replays_mark_what_they_change(bits):
             assert all(t._version > v for t, v in zip(tensors, seen))
             with pytest.raises(RuntimeError, match="modified by an inplace operation"):
                 late.backward()
+    torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("spare", [False, True])
+@pytest.mark.parametrize("bits", [32, 8])
+def test_a_parameter_at_rest_keeps_its_step_count(bits, spare):
+    """A parameter, first in the optimizer, that was trained for two steps and then frozen, or that the recorded step (the sixth) does not use: a
+    recording of the others goes on from their step count, not from its, and leaves it alone.  The same updates as eager ones, bit for bit."""
+    gen = torch.Generator(device=DEV).manual_seed(2)
+    x, y = (torch.randn(300, generator=gen, device=DEV) for _ in range(2))
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        models = [Tiny(bits), Tiny(bits)]
+        for model in models:
+            for i in range(5):
+                model.shape.requires_grad_(spare or i < 2)
+                model.training_step(x, y)
+            model.spare = spare
+        step = CapturedTrainingStep(models[0], x, y)
+        for count in (6, 7, 8):
+            step(x, y)
+            models[1].training_step(x, y)
+            for a, b in zip(models[0].parameters(), models[1].parameters()):
+                assert torch.equal(a.detach(), b.detach())
+            for model in models:
+                assert [int(model.optimizer.state[p]["step"]) for p in model.parameters()] == [5 if spare else 2, count, count]
     torch.cuda.synchronize()
