@@ -489,7 +489,7 @@ class CapturedTrainingStep:
             # the recording ran the step's Python (not its kernels): undo the one host-side effect, the step counters of what got a gradient
             self._trained = [p for p in trained if int(opt.state[p]["step"]) != self.step_count]
             self.sync_state()
-        self._changed = [t for p in self._trained for t in (p, *[opt.state[p][key] for key in opt._keys()])] if decoupled else []
+        self._places = self._where()
         stale = [w for w in caught if "AccumulateGrad" in str(w.message)]
         for w in caught:
             if w not in stale:
@@ -499,7 +499,17 @@ class CapturedTrainingStep:
             raise _lib.FscError("CapturedTrainingStep: a tensor of an earlier step's autograd graph is still alive (its AccumulateGrad "
                                 "nodes would run outside the recording); drop the previous steps' outputs before recording")
 
+    def _tensors(self):
+        """What the recorded optimizer step writes: parameters and moments as they are now."""
+        return [t for p in self._trained for t in (p, *self.opt.state[p].values()) if isinstance(t, torch.Tensor) and t.is_cuda]
+
+    def _where(self):
+        return list(map(torch.Tensor.data_ptr, self._tensors()))
+
     def __call__(self, signal, labels):
+        if self._where() != self._places:
+            raise _lib.FscError("CapturedTrainingStep: parameters or moments are not where they were recorded (a checkpoint loaded or the model moved "
+                                "since?); record the step again")
         if torch.cuda.current_stream(self.signal.device) != self.stream:
             raise _lib.FscError("CapturedTrainingStep: replay on the stream the step was recorded on")
         if tuple(signal.shape) != tuple(self.signal.shape) or tuple(labels.shape) != tuple(self.labels.shape):
@@ -525,7 +535,8 @@ class CapturedTrainingStep:
                 call("fsc_fill", to, float(value), 1, stream_ptr())
                 to += 4
         self.graph.replay()
-        _mark_changed(self._changed)
+        if isinstance(self.opt, FusedAdamW):
+            _mark_changed(self._tensors())
         return self.outputs
 
     def sync_state(self):

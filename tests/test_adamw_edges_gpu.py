@@ -9,6 +9,7 @@ pytestmark = pytest.mark.gpu
 if not torch.cuda.is_available():
     pytest.skip("needs an MI355X", allow_module_level=True)
 
+from freesound_classification_amd._lib import FscError  # noqa: E402
 from freesound_classification_amd.ops.training import CapturedTrainingStep, FusedAdamW  # noqa: E402
 
 DEV = "cuda:0"
@@ -82,4 +83,40 @@ def test_a_parameter_at_rest_keeps_its_step_count(bits, spare):
                 assert torch.equal(a.detach(), b.detach())
             for model in models:
                 assert [int(model.optimizer.state[p]["step"]) for p in model.parameters()] == [5 if spare else 2, count, count]
+    torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("change", ["checkpoint", "moment", "weight"])
+@pytest.mark.parametrize("bits", [32, 8])
+def test_a_recording_of_other_tensors_is_refused(bits, change):
+    """The recorded step writes where parameters and moments were: once they have been replaced (and the old ones may be somebody else's memory), it is
+    not replayed.  A checkpoint of the model, which is copied into place, is fine."""
+    gen = torch.Generator(device=DEV).manual_seed(4)
+    x, y = (torch.randn(300, generator=gen, device=DEV) for _ in range(2))
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        model = Tiny(bits)
+        model.training_step(x, y)
+        step = CapturedTrainingStep(model, x, y)
+        step(x, y)
+        model.load_state_dict({k: v.clone() for k, v in model.state_dict().items()})
+        step(x, y)
+        step.sync_state()
+        kept = model.weight.data, model.optimizer.state[model.weight]["exp_avg"]          # (so that the recording's memory stays what it was)
+        if change == "checkpoint":
+            old = [dict(st) for st in model.optimizer.state.values()]
+            model.optimizer.load_state_dict(model.optimizer.state_dict())
+            assert len(old) == 3
+        elif change == "moment":
+            model.optimizer.state[model.weight]["exp_avg"] = kept[1].clone()
+        else:
+            model.weight.data = kept[0].clone()
+        before = model.weight.detach().clone()
+        with pytest.raises(FscError, match="record the step again"):
+            step(x, y)
+        assert torch.equal(model.weight.detach(), before) and int(model.optimizer.state[model.weight]["step"]) == 3
+        again = CapturedTrainingStep(model, x, y)
+        again(x, y)
+        assert not torch.equal(model.weight.detach(), before) and int(model.optimizer.state[model.weight]["step"]) == 4
     torch.cuda.synchronize()
