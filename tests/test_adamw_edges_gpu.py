@@ -120,3 +120,45 @@ def test_a_recording_of_other_tensors_is_refused(bits, change):
         again(x, y)
         assert not torch.equal(model.weight.detach(), before) and int(model.optimizer.state[model.weight]["step"]) == 4
     torch.cuda.synchronize()
+
+
+def test_held_moments_are_right_in_the_mean():
+    """64 K elements beside one that is 9.3 times theirs in each block of 256 (the block's maximum: held exactly, as its scale), whose gradients then
+    fall tenfold.
+
+    The first moment is linear in what is held and rounding is right in the mean, so its mean is the true one within 5 deviations of a mean over the
+    elements.  The root: a step takes r to sqrt(beta2 r^2 + ...), which is convex, so a spread of s (relative to the mean) lifts the mean by s^2 / 2 at
+    most.  The spread: a code that falls by d is rounded to one of its neighbours, D apart, with a variance of d D; over a fall from code c0 to c1 that
+    is s^2 = the integral of (D / c) dlog(c), with 1/16 <= D / c <= 1/8 where codes are normal (above 2^-6), on top of what was there.  The second moment
+    that a step starts from is the root's square, so in the mean it is above the true one by that s^2: it is not right in the mean, the root is."""
+    count, steps = 1 << 16, (1000, 1500, 2500)
+    p = torch.nn.Parameter(torch.zeros(count, device=DEV))
+    opt = FusedAdamW([p], lr=0.0, weight_decay=0.0, state_bits=8, seed=5)
+    inner = torch.arange(count, device=DEV) % 256 != 0
+    many = int(inner.sum())
+    m = v = top = 0.0
+    was = None
+    for step in range(1, steps[-1] + 1):
+        g = 1.0 if step <= steps[0] else 0.1
+        p.grad = torch.where(inner, g, 9.3)
+        opt.step()
+        m, v, top = 0.9 * m + 0.1 * g, 0.999 * v + 0.001 * g * g, 0.999 * top + 0.001 * 9.3 ** 2
+        if step not in steps:
+            continue
+        st = opt.state[p]
+        held = (st["exp_avg"].float() * st["exp_avg_scale"].repeat_interleave(256))[inner].double()
+        assert abs(float(held.mean()) - m) <= 5 * float(held.std()) / many ** 0.5
+        root = (st["exp_avg_sq_root"].float() * st["exp_avg_sq_root_scale"].repeat_interleave(256))[inner].double()
+        mean, code = float(root.mean()), 448 * (v / top) ** 0.5
+        spread2 = float(root.var()) / mean ** 2
+        luck = 5 * (spread2 / many) ** 0.5
+        assert abs(mean / v ** 0.5 - 1) <= spread2 / 2 + luck, (step, mean / v ** 0.5)
+        if was is None:
+            was = spread2, code
+            assert spread2 < 1 / 8 ** 2 and code > 32                # (at rest between two neighbours at most 1 / 8 apart)
+        else:
+            fall = torch.log(torch.tensor(was[1] / code)).item()
+            few = 5 * (2 / many) ** 0.5 * spread2                   # (of an estimated variance)
+            assert fall / 16 - few <= spread2 <= was[0] + fall / 8 + few, (step, spread2, fall)
+        excess = float(root.square().mean()) / v - 1
+        assert abs(excess - spread2) <= (spread2 + 2 * luck) * (1 + spread2), (step, excess)
