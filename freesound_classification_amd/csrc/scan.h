@@ -288,11 +288,11 @@ __device__ __forceinline__ void scan_rates(const fsc_selective_scan_args& a, con
     for (int i = 0; i < NS; ++i) rate[i] = w.real && w.sg * NS + i < a.states ? rate_of(rate[i]) : 0.f;
 }
 
-// A state behind a segment: what was in front of it times the segment's decay, and the segment's end from zero.  An infinity outlasts every decay, also
-// one that is 0 in fp32 (frame by frame it meets factors above 0), unless a time step itself was infinite.
+// A state behind a segment: what was in front of it times the segment's decay, and the segment's end from zero.  An infinity outlasts a decay that is 0
+// in fp32: frame by frame it meets factors above 0.
 __device__ __forceinline__ float scan_join(float h, float rate, float sum_delta, float end) {
-    const float decay = __builtin_amdgcn_exp2f(rate * sum_delta);
-    return fabsf(h) == INFINITY && sum_delta < INFINITY ? h + end : fmaf(decay, h, end);
+    const float joined = fmaf(__builtin_amdgcn_exp2f(rate * sum_delta), h, end);
+    return joined == joined ? joined : h + end;
 }
 
 // The lane's states of a (batch, channels, states) tensor, zeros without one.

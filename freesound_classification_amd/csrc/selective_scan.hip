@@ -35,7 +35,7 @@ __global__ __launch_bounds__(256) void scan_fwd_kernel(fsc_selective_scan_args a
             float e[NS];
             load_row<NS>(ends + w.end(p, q), true, NS, e);
 #pragma unroll
-            for (int i = 0; i < NS; ++i) h[i] = w.sg * NS + i < a.states ? scan_join(h[i], rate[i], ds, e[i]) : 0.f;
+            for (int i = 0; i < NS; ++i) h[i] = scan_join(h[i], rate[i], ds, e[i]);
         }
     }
     float bias[E], skip[E];

@@ -156,7 +156,7 @@ __global__ __launch_bounds__(256, 2) void scan_bwd_kernel(fsc_selective_scan_arg
         float more[NS];
         load_row<NS>(ws + at.ends + w.end(p, q), true, NS, more);
 #pragma unroll
-        for (int i = 0; i < NS; ++i) e[i] = w.real && w.sg * NS + i < a.states ? scan_join(e[i], rate[i], ds, more[i]) : 0.f;
+        for (int i = 0; i < NS; ++i) e[i] = scan_join(e[i], rate[i], ds, more[i]);
     }
     float bias[E], skip[E], dskip[E] = {}, dbias[E] = {};
     scan_param(w, a.dt_bias, bias);
