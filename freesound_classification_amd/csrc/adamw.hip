@@ -3,13 +3,15 @@
 //   g = grad * grad_scale;  m = m beta1 + g (1 - beta1);  v = v beta2 + (g g)(1 - beta2);  r = sqrt(v)
 //   p = p decay - (m / (r inv_root + eps)) step_size
 // Bound: HBM.  32-bit moments: 28 bytes a parameter in fp32 (p, g, m, v read; p, m, v written); 8-bit moments: 16, 10 in bf16.
-// 21 M parameters in 141 tensors: 107 us with 32 bits (5.5 TB/s; part of it stays in the last-level cache), 75 with 8; 200 M in bf16 with 8 bits: 500 us
-// (4.1 TB/s, and some 75 vector instructions an element).
+// 21 M parameters in 141 tensors: 107 us with 32 bits (5.5 TB/s, above what HBM gives: part of it stays in the last-level cache), 75 with 8; 200 M in bf16
+// with 8 bits: 510 us (3.9 TB/s, and some 75 vector instructions an element).
 //
 // 8-bit moments.  m and r = sqrt(v) (half the decades of v) are held as e4m3 values of x / scale, scale = the largest |x| of 256
 // consecutive elements / 448.  Rounding to nearest would freeze them: beta2 = 0.999 moves v by 0.1 % a step and half a step of e4m3 is
-// 6 %.  So a value is rounded down or up with the probability of its remainder, from 16 bits of a hash of (salt, step, element): the mean
-// moves as in 32 bits.  r > 0 is never held as 0 -- its next step would divide by eps.
+// 6 %.  So a value is rounded down or up with the probability of its remainder, from 16 bits of a hash of (salt, step, element): the means of m and
+// r move as in 32 bits.  The mean of v = r^2 does not: rounding spreads r, and v is above its true mean by that variance -- under 0.5 % where gradients
+// keep their size; where an element's fall against its block's largest, by the logarithm of the fall / 16 to / 8 (tenfold, over 1500 steps: 7 %).
+// r > 0 is never held as 0 -- its next step would divide by eps.
 // One wave owns a block of 256: four elements a lane, the block's maximum through lane exchanges, no LDS.
 #include <math.h>
 

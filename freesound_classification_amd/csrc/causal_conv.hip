@@ -5,8 +5,8 @@
 // neighbouring threads read neighbouring channels.  Frames are taken eight at a time, all their loads issued before the first is used.
 // Backward: the strip recomputes pre (cheaper than keeping it) and runs K - 1 frames past its end; dw / db are summed in registers, over
 // the block's strips through LDS, over blocks by a second launch in a fixed order: equal inputs give equal bits.
-// 4 x 8191 x 2048 in bf16, ragged (80 % of the frames), x a half of a wider tensor: forward 53 us (4.5 TB/s, what a copy of this size reaches), backward 93
-// (3.7 TB/s: two waves a SIMD, the window, its gradient and the filters' sums fill the registers).  128 x 53 x 256 in fp32: 6.5 and 17 us.
+// 4 x 8191 x 2048 in bf16, ragged (80 % of the frames), x a half of a wider tensor: forward 53 us (4.6 TB/s, what a copy of this size reaches), backward 90
+// + 4 (3.8 TB/s: two waves a SIMD, the window, its gradient and the filters' sums fill the registers).  128 x 53 x 256 in fp32: 6.5 and 17 us.
 #include <type_traits>
 
 #include "seq.h"
@@ -199,11 +199,12 @@ __global__ __launch_bounds__(kThreads) void conv_bwd_kernel(fsc_causal_conv_args
         for (int j = 0; j < K - 1; ++j)
 #pragma unroll
             for (int i = 0; i < V; ++i) dp[j][i] = 0.f;
-        // frame t yields d pre[t]; with it frame t - (K - 1) has its gradient.  The next U frames are on their way while these are worked on:
-        // with two waves a SIMD nothing else covers the loads (4 x 8191 x 2048 in bf16: 97 us, 120 where each load was waited for at once)
+        // Frame t yields d pre[t]; with it frame t - (K - 1) has its gradient.  The next U frames are on their way while these are worked on: where
+        // there are two waves a SIMD, little else covers the loads (4 x 8191 x 2048 in bf16, forward and backward: 8 taps 185 us, 278 with the loads at
+        // the start of their turn, which also keeps more registers; 5 taps 147 for 160; up to 4 taps as long either way)
         fsc::Raw<T, V> raw_x[U] = {}, raw_dy[U] = {};
         auto ahead = [&](int t) {
-            if (t < len) {       // (behind the end the last values stay, or the zeros: their gradient is 0 and must meet a number)
+            if (t < len) {       // (behind the end the last values stay, or the zeros: what comes of them is left out)
                 fetch<T, V, U>(a.x, a.x_batch, a.x_time, n, c, t, len, wide, have, raw_x);
                 if (a.dy != nullptr) fetch<T, V, U>(a.dy, a.dy_batch, a.dy_time, n, c, t, len, wide, have, raw_dy);
             }
@@ -268,7 +269,7 @@ __global__ __launch_bounds__(kThreads) void conv_bwd_kernel(fsc_causal_conv_args
                         for (int i = 0; i < V; ++i) dx[i] += more[i];
                     }
                 }
-                if (j == U - 1) {                    // (95 us for 97)
+                if (j == U - 1) {                    // (in front of this turn's last store: backward of 4 taps 90 us for 92)
 #pragma unroll
                     for (int q = 0; q < U; ++q) {
                         raw_x[q].arrived();
@@ -390,8 +391,8 @@ Plan plan(const fsc_causal_conv_args& a) {
     return p;
 }
 
-// Blocks along the rows of the backward pass: two blocks a CU, as many as the registers let in (4 x 8191 x 2048 in bf16: 116 us, with four
-// 120), and no more partial sums than that.
+// Blocks along the rows of the backward pass: two blocks a CU, as many as the registers let in (4 x 8191 x 2048 in bf16: 90 us; four 97, one 121),
+// and no more partial sums than that.
 int bwd_parts(const Plan& p) {
     if (p.groups == 0) return 1;                 // no channels: nothing is launched
     const int across = fsc::ceil_div(p.groups, p.lanes), need = fsc::ceil_div(p.rows, kThreads / p.lanes);

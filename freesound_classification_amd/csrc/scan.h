@@ -9,8 +9,8 @@
 //     ([channel][frame]), B / C a row a frame; the sum over the states is NS multiply-adds and log2 L lane exchanges.
 // Where sequences x channel blocks do not fill the card, time is cut into segments: a first launch computes each segment's end from zero
 // (and the sum of its delta: exp(A sum) is the segment's decay), the main launch joins the ends in front of its own segment.
-// Measured with 16 states, bf16, ragged: 2 x 16384 frames of 2048 channels 252 us + 177 for the ends (9 vector instructions an element, 5 of them the
-// recurrence); 8 x 2048 of 1024 channels 71 + 50, backward 215 + 54 (19 instructions an element; h and exp(delta A) of a tile's frames take half the
+// Measured with 16 states, bf16, ragged: 2 x 16384 frames of 2048 channels 255 us + 177 for the ends (9 vector instructions an element, 5 of them the
+// recurrence); 8 x 2048 of 1024 channels 72 + 49, backward 225 + 54 (19 instructions an element; h and exp(delta A) of a tile's frames take half the
 // registers and leave two waves a SIMD).
 #pragma once
 #include "seq.h"
@@ -46,8 +46,8 @@ inline ScanPlan scan_plan(const fsc_selective_scan_args& a) {
     p.blocks = a.groups * p.group_blocks;
     p.tiles = ceil_div(a.length, kTile);
     // 1024 workgroups are four waves a SIMD (a long training step, 8 x 2048 frames of 1024 channels, forward + its ends | backward + its ends:
-    // 512: 151 | 311 us, 1024: 121 | 268, 2048: 122 | 276).  Segments double the exponentials, so half of that is enough not to cut (a batch of 128 x
-    // 53 frames of 256 channels, 512 workgroups: 19 | 39 us whole, 31 | 62 cut in two).
+    // 512: 151 | 309 us, 1024: 122 | 275, 2048: 128 | 293).  Segments double the exponentials, so half of that is enough not to cut (a batch of 128 x
+    // 53 frames of 256 channels, 512 workgroups: 19 | 40 us whole, 30 | 61 cut in two).
     const long have = (long)a.batch * p.blocks, wanted = 1024;
     p.segments = 1;
     if (have > 0 && have * 2 < wanted && p.tiles >= 4) {        // (no sequences or no channels: nothing to cut)

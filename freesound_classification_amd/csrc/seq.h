@@ -140,7 +140,7 @@ __device__ __forceinline__ void swap16(float& a, float& b) {
 
 inline size_t dtype_bytes(int dtype) { return dtype == FSC_DTYPE_F32 ? 4 : 2; }
 inline bool dtype_ok(int dtype) { return dtype == FSC_DTYPE_F32 || dtype == FSC_DTYPE_BF16 || dtype == FSC_DTYPE_F16; }
-// whether `bytes`-wide accesses at p + multiples of `strides` elements stay aligned
+// whether p is a multiple of `bytes`, a power of two
 inline bool aligned(const void* p, size_t bytes) { return ((uintptr_t)p & (bytes - 1)) == 0; }
 
 }  // namespace fsc

@@ -100,7 +100,7 @@ class SsmHead(nn.Module):
     def _mark(self):
         self.a_log.no_decay = self.d.no_decay = True
 
-    def __setstate__(self, state):                           # (copy.deepcopy and torch.load make parameters without the mark)
+    def __setstate__(self, state):                           # (copy.deepcopy makes parameters without the mark)
         super().__setstate__(state)
         self._mark()
 

@@ -158,9 +158,11 @@ class FusedAdamW(Optimizer):
     `state_bits=32`: state keys match torch (step, exp_avg, exp_avg_sq), moments in fp32.  `state_bits=8`: the moments are held as e4m3 values
     with one fp32 scale per 256 elements -- exp_avg / exp_avg_scale, and the square root of the second moment, exp_avg_sq_root /
     exp_avg_sq_root_scale --, 2.03 bytes a parameter instead of 8, rounded stochastically: the random bits are a function of (`seed`, the
-    tensor's place in the optimizer, the step, the element), so a run is reproducible.  Parameters and gradients are fp32, bf16 or fp16.
-    `grad_scale` multiplies gradients first (1 / world_size after a summing all-reduce).  A refused step changes nothing in its group; a
-    step is recorded into a HIP graph by CapturedTrainingStep alone (elsewhere the step count would be frozen into it)."""
+    tensor's place in the optimizer, the step, the element), so a run is reproducible.  The means of the first moment and of the root are the
+    true ones; the second moment, the root's square, is above its own by the variance of the rounding (under 0.5 %, more where an element's
+    gradients shrink against its neighbours').  Parameters and gradients are fp32, bf16 or fp16.
+    `grad_scale` multiplies gradients first (1 / world_size after a summing all-reduce).  A refused step changes nothing in its group, a
+    refused checkpoint nothing at all; a step is recorded into a HIP graph by CapturedTrainingStep alone (elsewhere the step count would be frozen into it)."""
 
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, state_bits=32, seed=0):
         if state_bits not in (32, 8):
