@@ -5,7 +5,7 @@
 // neighbouring threads read neighbouring channels.  Frames are taken eight at a time, all their loads issued before the first is used.
 // Backward: the strip recomputes pre (cheaper than keeping it) and runs K - 1 frames past its end; dw / db are summed in registers, over
 // the block's strips through LDS, over blocks by a second launch in a fixed order: equal inputs give equal bits.
-// 4 x 8191 x 2048 in bf16, ragged (80 % of the frames), x a half of a wider tensor: forward 53 us (4.6 TB/s, what a copy of this size reaches), backward 90
+// 4 x 8191 x 2048 in bf16, ragged (80 % of the frames), x a half of a wider tensor: forward 53 us (4.6 TB/s, what a copy of this size reaches), backward 90 - 95
 // + 4 (3.8 TB/s: two waves a SIMD, the window, its gradient and the filters' sums fill the registers).  128 x 53 x 256 in fp32: 6.5 and 17 us.
 #include <type_traits>
 

@@ -5,7 +5,8 @@ and for single frames over a kept state.  Public through `functional` (`causal_c
 Sequences are (N, T, D) with the channels last; tensors whose channels are contiguous are read in place whatever the strides of their other
 axes (halves of one projection, time slices), others are copied first.  Activations are fp32, bf16 or fp16 (one type per call), parameters and
 scan states fp32; sums and states are fp32 inside, with one rounding at each output.  `lengths` (N,) int32 marks padded batches: frames at and
-behind lengths[n] are never read (they may hold anything), give zeros and get zero gradients, and states pass them by unchanged.
+behind lengths[n] are never read (they may hold anything), give zeros and get zero gradients, and states pass them by unchanged.  Infinities and NaN in
+frames that exist go where the formulas take them and nowhere else.  First derivatives only, backwards only: others are refused.
 """
 import torch
 from torch.autograd import forward_ad

@@ -649,7 +649,8 @@ int fsc_sgd_nesterov_step(const fsc_opt_tensor* tensors_host, int n_tensors, flo
  * state_bits 32: state0 = m, state1 = v (fp32).  state_bits 8: state0 / state1 = e4m3 values of m / sqrt(v), scale0 / scale1 one fp32
  * scale for each 256 elements; each value is rounded down or up with the probability of its remainder, from 16 bits of a counter-based
  * hash of (salt, step modulo 2^24, element), and a second moment above 0 is never held as 0.  A value that is not finite is held as NaN
- * and leaves its block's scale alone. */
+ * and leaves its block's scale alone.  (In the mean over the random bits state0 and state1 are the exact averages; the square of state1 is above
+ * the second moment by its variance.) */
 typedef struct {
     void* param;
     const void* grad;
