@@ -333,11 +333,13 @@ void with_scan_shape(const ScanPlan& p, Fn fn) {
     else fn(std::integral_constant<int, 4>(), std::integral_constant<int, 1>());
 }
 
-// fn(flag) with the flag as a type
-template <typename Fn>
-void with_flag(bool flag, Fn fn) {
-    if (flag) fn(std::true_type());
-    else fn(std::false_type());
+// fn(partial) with, as a type, whether some lane has fewer states than its NS
+template <int NS, typename Fn>
+void with_partial(int states, Fn fn) {
+    if constexpr (NS > 1) {
+        if (states % NS != 0) return fn(std::true_type());
+    }
+    fn(std::false_type());
 }
 
 }  // namespace fsc

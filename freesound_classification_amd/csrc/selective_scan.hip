@@ -217,7 +217,7 @@ int fsc_selective_scan_fwd(const fsc_selective_scan_args* args_host, fsc_stream_
         using T = decltype(type);
         with_scan_shape(p, [&](auto lanes, auto per) {
             constexpr int L = decltype(lanes)::value, NS = decltype(per)::value;
-            with_flag(a.states % NS != 0, [&](auto partial) {
+            with_partial<NS>(a.states, [&](auto partial) {
                 constexpr bool PARTIAL = decltype(partial)::value;
                 if (p.segments > 1)
                     hipLaunchKernelGGL((scan_fwd_kernel<T, L, NS, true, PARTIAL>), grid, dim3(256), 0, as_stream(stream), a, p, ends, end_deltas);

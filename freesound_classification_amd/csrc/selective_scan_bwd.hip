@@ -445,7 +445,7 @@ int fsc_selective_scan_bwd(const fsc_selective_scan_args* args_host, fsc_stream_
         if (a.batch > 0 && a.channels > 0)               // (without channels db and dc are still there: sums over nothing)
             with_scan_shape(p, [&](auto lanes, auto per) {
                 constexpr int L = decltype(lanes)::value, NS = decltype(per)::value;
-                with_flag(a.states % NS != 0, [&](auto partial) {
+                with_partial<NS>(a.states, [&](auto partial) {
                     constexpr bool PARTIAL = decltype(partial)::value;
                     if (p.segments > 1)
                         hipLaunchKernelGGL((scan_bwd_ends_kernel<T, L, NS, PARTIAL>), grid, dim3(256), 0, as_stream(stream), a, p, ws + at.ends,
